@@ -53,7 +53,9 @@ def permute(ids: torch.Tensor, num_experts: int, workspace: Optional[torch.Tenso
     N = ids.numel()
     L = _lib.lib()
     gs = torch.empty(num_experts, dtype=torch.int32, device=dev)
-    src = torch.empty(N, dtype=torch.int32, device=dev)
+    # Rows past sum(group_sizes), which dropped entries leave over, read as
+    # entry 0: gather_rows takes every row of sorted_src.
+    src = torch.zeros(N, dtype=torch.int32, device=dev)
     inv = torch.empty(ids.shape, dtype=torch.int32, device=dev)
     need = int(L.moe_permute_workspace_size(N, num_experts))
     if workspace is None or workspace.numel() < need:
