@@ -401,6 +401,105 @@ int moe_fused_mlp_swiglu_backward(const void* x, const void* w_gate_up, const vo
                                   float* dx, float* dw_gate_up, float* dw_down, int64_t M, int32_t D, int32_t F,
                                   int32_t E, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Training of a whole MoE layer: the steps around the expert MLP's backward.
+ * No counterpart in the reference (forward-only, and its path starts from
+ * sorted rows).  Element types of logits, row gradients and gradient lists:
+ */
+enum { MOE_ELEM_F32 = 0, MOE_ELEM_BF16 = 1, MOE_ELEM_F16 = 2 };
+enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
+
+/*
+ * Top-k routing with its auxiliary losses.  logits (T, E) of elem_type, rows
+ * ld >= E elements apart; the T tokens are `sequences` runs of equal length
+ * (T a multiple of it).  With p = softmax(l), s = sigmoid(l) per token and q =
+ * p (softmax scoring) or s / sum(s) (sigmoid scoring):
+ *   ids      (T, k) int32: the k largest logits, ties to the lower expert id;
+ *            -1 where no logit above -inf is left (NaN is never chosen)
+ *   weights  (T, k) f32: scores (p or s) of the chosen experts, divided by
+ *            their sum when `normalize`; 0 at id -1
+ *   counts   (sequences, E) int32 c: chosen entries per expert
+ *   tokens   (sequences,) int32 N: tokens that take part
+ *   balance  f32: mean over the sequences with tokens of
+ *            sum_e (c_e E / (k N)) (sum_t q_te / N)
+ *   z        f32: mean over tokens of logsumexp(l)^2
+ * mask (T,) bytes or NULL: a token whose byte is 0, or whose logits are all
+ * -inf or NaN, takes no part: ids -1, weights 0, no share in any sum.
+ * given_ids (T, k) or NULL: experts chosen by the caller, used in place of the
+ * top k (an id outside [0, E) counts as -1; one id may come up twice).
+ * E <= 1024, k <= min(16, E), T k < 2^31.  A NaN logit of a token that takes
+ * part makes the losses NaN.  Workspace: moe_route_train_workspace_size
+ * bytes, 256-byte aligned.
+ *
+ * moe_route_backward: d_logits (T, E) contiguous, of elem_type, for the
+ * upstream gradients d_weights (T, k) f32, d_balance and d_z (device f32
+ * scalars), each of which may be NULL (zero).  ids, weights, counts and
+ * tokens are the forward's; mask, scoring and normalize as given there.
+ * Tokens that take no part, and logits of -inf, get 0.
+ */
+size_t moe_route_train_workspace_size(int64_t T, int32_t E, int64_t sequences);
+int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
+                    int64_t sequences, const uint8_t* mask, const int32_t* given_ids, int32_t scoring,
+                    int32_t normalize, int32_t* ids, float* weights, int32_t* counts, int32_t* tokens, float* balance,
+                    float* z, void* workspace, size_t workspace_bytes, void* stream);
+int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
+                       int64_t sequences, const uint8_t* mask, int32_t scoring, int32_t normalize, const int32_t* ids,
+                       const float* weights, const int32_t* counts, const int32_t* tokens, const float* d_weights,
+                       const float* d_balance, const float* d_z, void* d_logits, void* stream);
+
+/*
+ * Backward of moe_combine_rows and moe_gather_rows.  inverse (T, k) is
+ * moe_permute's: the row of each entry, -1 (or any value outside [0, rows))
+ * for a dropped one; no row comes up twice.  D a multiple of 4; row tensors
+ * 16-byte aligned (8-byte for the 16-bit types).
+ *
+ * moe_combine_rows_backward  y_sorted (rows, D) f32, dy (T, D) of dy_type ->
+ *                  dys (rows, D) of dys_type: dys[inverse[t, j]] =
+ *                  weights[t, j] dy[t], rows past sum(group_sizes) zero; and
+ *                  dw (T, k) f32 = <dy[t], y_sorted[inverse[t, j]]>, 0 where
+ *                  dropped.
+ * moe_gather_rows_backward   dxs (rows, D) of dxs_type -> dx (T, D) of
+ *                  dx_type: the f32 sum of dxs[inverse[t, j]] in slot order.
+ */
+int moe_combine_rows_backward(const void* dy, int32_t dy_type, const float* y_sorted, const int32_t* inverse,
+                              const float* weights, const int32_t* group_sizes, int64_t T, int32_t k, int32_t D,
+                              int64_t rows, int32_t E, void* dys, int32_t dys_type, float* dw, void* stream);
+int moe_gather_rows_backward(const void* dxs, int32_t dxs_type, const int32_t* inverse, int64_t T, int32_t k,
+                             int32_t D, int64_t rows, void* dx, int32_t dx_type, void* stream);
+
+/*
+ * Norm of a list of tensors taken as one vector, and their scaling to a
+ * largest norm.  A tensor is rows x cols elements with rows in_ld (in) and
+ * out_ld (out) elements apart; dense tensors of any shape are one row.  The
+ * descriptors are host memory, read during the call; n may be 0.
+ *
+ * moe_grad_norm    *norm (device f32) = (sum |x|^p)^(1/p) over all tensors;
+ *                  `out` is not used.  Sums run in f64 across groups of 32
+ *                  elements: no overflow or underflow below f32's own.
+ * moe_clip_grads   out = in * min(1, max_norm / (norm + 1e-6)) in f32, rounded
+ *                  once to out_type.  given_norm (device f32): the norm to use
+ *                  (one that was reduced over ranks, say); NULL: computed
+ *                  here.  norm (device f32, or NULL with a given norm)
+ *                  receives the norm.  `out` may be `in` (same type and
+ *                  strides), and then nothing is written when the factor is
+ *                  1; otherwise an `out` overlaps no tensor of the list.  A
+ *                  NaN norm makes every output NaN, an infinite one 0 (NaN
+ *                  where the element is infinite).
+ * Workspace: moe_grad_norm_workspace_size(n) bytes, 256-byte aligned.
+ */
+enum { MOE_NORM_L1 = 1, MOE_NORM_L2 = 2, MOE_NORM_INF = 3 };
+typedef struct moe_tensor_desc {
+  const void* in;
+  void* out;
+  int64_t rows, cols, in_ld, out_ld;
+  int32_t in_type, out_type; /* MOE_ELEM_* */
+} moe_tensor_desc;
+size_t moe_grad_norm_workspace_size(int32_t n);
+int moe_grad_norm(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int moe_clip_grads(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type, double max_norm,
+                   const float* given_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Text of the calling thread's last error ("" when none). */
 const char* moe_last_error(void);
 

@@ -361,3 +361,137 @@ def ref_ragged_swiglu_backward(x: np.ndarray, w_gate: np.ndarray, w_up: np.ndarr
         dwu[e] = xe.T @ du
         dwd[e] = (g * s * u).T @ ye
     return dx, dwg, dwu, dwd
+
+
+# ----------------------------------------------------------------------------- training of a whole layer
+# No counterpart in the reference (forward-only; its path starts from sorted
+# rows).  Definitions in float64 of the steps around the expert MLP's backward.
+
+def route_train(logits: np.ndarray, k: int, ids=None, mask=None, sequences: int = 1, scoring: str = "softmax",
+                normalize: bool = True) -> dict:
+    """Top-k routing with the balance and z losses: ids, weights, counts,
+    tokens, balance, z, and the quantities its gradient is made of (p, q,
+    slope = d log(score)/d logit over softmax's, lse, keep, f = c E / (k N))."""
+    x = np.asarray(logits, np.float64)
+    T, E = x.shape
+    S, L = sequences, T // sequences
+    keep = np.zeros(T, bool)
+    for t in range(T):
+        keep[t] = np.any(x[t] > -np.inf) and (mask is None or bool(mask[t]))
+    p, q, slope, score = (np.zeros((T, E)) for _ in range(4))
+    lse = np.zeros(T)
+    out_ids = np.full((T, k), -1, np.int32)
+    weights = np.zeros((T, k))
+    counts = np.zeros((S, E), np.int64)
+    tokens = np.zeros(S, np.int64)
+    for t in np.flatnonzero(keep):
+        row = x[t]
+        m = np.nanmax(row)
+        e = np.exp(row - m)
+        p[t] = e / e.sum()
+        lse[t] = m + np.log(e.sum())
+        if scoring == "softmax":
+            score[t], q[t], slope[t] = p[t], p[t], 1.0
+        else:
+            low = np.logaddexp(0.0, -row)              # -log(sigmoid)
+            score[t] = np.exp(-low)
+            rel = np.exp(low.min() - low)
+            q[t] = rel / rel.sum()
+            slope[t] = np.exp(-np.logaddexp(0.0, row))
+        if ids is None:
+            order = sorted((e for e in range(E) if row[e] > -np.inf), key=lambda e: (-row[e], e))[:k]
+            out_ids[t, :len(order)] = order
+        else:
+            out_ids[t] = [i if 0 <= i < E else -1 for i in np.asarray(ids[t])]
+        on = out_ids[t] >= 0
+        at = out_ids[t][on]
+        if normalize and len(at):
+            # On the chosen experts' own scale, so that no row of small scores is lost.
+            ls = row[at] - lse[t] if scoring == "softmax" else -np.logaddexp(0.0, -row[at])
+            if np.max(ls) > -np.inf:
+                w = np.exp(ls - np.max(ls))
+                weights[t][on] = w / w.sum()
+        else:
+            weights[t][on] = score[t][at]
+        tokens[t // L] += 1
+        np.add.at(counts[t // L], at, 1)
+    n = np.maximum(tokens, 1)[:, None]
+    f = counts * E / (k * n)
+    mean_q = q.reshape(S, L, E).sum(1) / n
+    live = max(int((tokens > 0).sum()), 1)
+    balance = float((f * mean_q).sum() / live)
+    total = max(int(tokens.sum()), 1)
+    z = float((lse[keep] ** 2).sum() / total)
+    return {"ids": out_ids, "weights": weights, "counts": counts, "tokens": tokens, "balance": balance, "z": z, "p": p,
+            "q": q, "slope": slope, "lse": lse, "keep": keep, "f": f, "live": live, "total": total,
+            "normalize": normalize, "scoring": scoring, "seq_len": L, "k": k}
+
+
+def route_train_backward(r: dict, d_weights=None, d_balance: float = 0.0, d_z: float = 0.0):
+    """(gradient, scale) with respect to the logits of ``route_train``'s
+    result: scale is the sum of the absolute values of what each element is
+    computed from, the measure of its rounding error."""
+    T, E = r["p"].shape
+    d = np.zeros((T, E))
+    scale = np.zeros((T, E))
+    for t in np.flatnonzero(r["keep"]):
+        s = t // r["seq_len"]
+        p, q, slope = r["p"][t], r["q"][t], r["slope"][t]
+        f = r["f"][s] - 1.0
+        b = d_balance / (r["live"] * r["tokens"][s])
+        d[t] = b * q * slope * (f - (f * q).sum()) + d_z * 2 * r["lse"][t] / r["total"] * p
+        scale[t] = (abs(b) * q * slope * (np.abs(f) + (np.abs(f) * q).sum())
+                    + abs(d_z) * 2 * abs(r["lse"][t]) / r["total"] * p)
+        if d_weights is None:
+            continue
+        on = r["ids"][t] >= 0
+        at, w, dw = r["ids"][t][on], r["weights"][t][on], np.asarray(d_weights[t], np.float64)[on]
+        dot, adot = (w * dw).sum(), (w * np.abs(dw)).sum()
+        if r["normalize"]:
+            np.add.at(d[t], at, w * (dw - dot) * slope[at])
+            np.add.at(scale[t], at, w * (np.abs(dw) + adot) * slope[at])
+        else:
+            np.add.at(d[t], at, w * dw * slope[at])
+            np.add.at(scale[t], at, w * np.abs(dw) * slope[at])
+            if r["scoring"] == "softmax":
+                d[t] -= p * dot
+                scale[t] += p * adot
+    return d, scale
+
+
+def combine_rows_backward(dy, y_sorted, inverse, weights):
+    """(dys, dw) of ``combine_rows``: rows that no entry maps to are zero."""
+    dy, ys = np.asarray(dy, np.float64), np.asarray(y_sorted, np.float64)
+    dys = np.zeros_like(ys)
+    dw = np.zeros(inverse.shape)
+    for t, j in zip(*np.nonzero((inverse >= 0) & (inverse < len(ys)))):
+        dys[inverse[t, j]] = weights[t, j] * dy[t]
+        dw[t, j] = dy[t] @ ys[inverse[t, j]]
+    return dys, dw
+
+
+def gather_rows_backward(dxs, inverse):
+    """dx[t] = the sum of the rows its entries map to."""
+    dxs = np.asarray(dxs, np.float64)
+    dx = np.zeros((inverse.shape[0], dxs.shape[1]))
+    for t, j in zip(*np.nonzero((inverse >= 0) & (inverse < len(dxs)))):
+        dx[t] += dxs[inverse[t, j]]
+    return dx
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> float:
+    """Norm of all arrays taken as one vector."""
+    parts = [np.abs(np.asarray(g, np.float64)).reshape(-1) for g in grads]
+    v = np.concatenate(parts) if parts else np.zeros(0)
+    if v.size == 0:
+        return 0.0
+    if norm_type == np.inf:
+        return float(np.max(v)) if not np.isnan(v).any() else float("nan")
+    return float(v.sum()) if norm_type == 1 else float(np.sqrt((v * v).sum()))
+
+
+def clip_grads(grads, max_norm: float, norm: float):
+    """The arrays times min(1, max_norm / (norm + 1e-6))."""
+    ratio = max_norm / (norm + 1e-6)
+    coef = 1.0 if ratio >= 1.0 else ratio
+    return [np.asarray(g, np.float64) * coef for g in grads]

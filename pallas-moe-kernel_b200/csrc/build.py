@@ -18,7 +18,8 @@ PKG = CSRC.parent
 REPO = PKG.parent
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libmoe_b200.so"
-SOURCES = ["moe_b200.cu"]
+OBJ_DIR = PKG / "_build"
+SOURCES = ["moe_b200.cu", "layer_train.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -42,12 +43,25 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if all(p.stat().st_mtime <= lib_t for p in _deps()):
             return LIB
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-shared",
-           "-I", str(REPO / "include"), "-o", str(tmp), *[str(CSRC / s) for s in SOURCES]]
+    OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    flags = [*ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-I", str(REPO / "include")]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True, cwd=str(CSRC))
+        flags.insert(0, "-Xptxas=-v")
+    newest_header = max(p.stat().st_mtime for p in _deps() if p.suffix != ".cu")
+    jobs, objects = [], []
+    for name in SOURCES:  # one nvcc per source, side by side; objects newer than their inputs are kept
+        src, obj = CSRC / name, OBJ_DIR / (name + ".o")
+        objects.append(str(obj))
+        if not force and obj.exists() and obj.stat().st_mtime > max(newest_header, src.stat().st_mtime):
+            continue
+        cmd = [_nvcc(), *flags, "-c", "-o", str(obj), str(src)]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        jobs.append((cmd, subprocess.Popen(cmd, cwd=str(CSRC))))
+    for cmd, job in jobs:
+        if job.wait():
+            raise subprocess.CalledProcessError(job.returncode, cmd)
+    subprocess.run([_nvcc(), *ARCH, "-shared", "-o", str(tmp), *objects], check=True, cwd=str(CSRC))
     os.replace(tmp, LIB)
     return LIB
 

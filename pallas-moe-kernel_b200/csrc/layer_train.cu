@@ -1,0 +1,505 @@
+// C ABI of the steps that train a whole MoE layer around its expert MLP:
+// top-k routing with the balance and z losses, the backward of the row
+// movement, and gradient norms and clipping.  Declarations:
+// include/moe_b200.h.
+#include <algorithm>
+#include <cstring>
+
+#include "abi_util.h"
+#include "grad_norm.cuh"
+#include "router_train.cuh"
+#include "row_grads.cuh"
+
+namespace moe {
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static size_t elem_bytes(int type) { return type == MOE_ELEM_F32 ? 4 : 2; }
+static bool elem_ok(int type) { return type == MOE_ELEM_F32 || type == MOE_ELEM_BF16 || type == MOE_ELEM_F16; }
+
+// ------------------------------------------------------------------ routing
+// Lanes per row: 8 experts a lane up to 256 experts (a 16-byte vector of the
+// 16-bit types), then the whole warp with more experts a lane.
+static int route_lanes(int E) {
+  int g = 1;
+  while (g < 32 && g * 8 < E) g *= 2;
+  return g;
+}
+
+// Blocks per sequence: enough that a warp has one step of tokens, and at most
+// kRouteBlocks over all sequences where a sequence is longer than that.
+constexpr int64_t kRouteBlocks = 148 * 2;
+static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
+  const int64_t step = kRouteWarps * (32 / route_lanes(E));
+  const int64_t most = std::max<int64_t>(1, kRouteBlocks / std::max<int64_t>(1, sequences));
+  return std::max<int64_t>(1, std::min((seq_len + step - 1) / step, most));
+}
+
+struct RouteSpace {
+  size_t q, c, z, n, seq, ticket, bytes;
+};
+static RouteSpace route_space(int64_t blocks, int64_t sequences, int E) {
+  RouteSpace s;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  s.q = take((size_t)blocks * E * sizeof(float));
+  s.c = take((size_t)blocks * E * sizeof(int32_t));
+  s.z = take((size_t)blocks * sizeof(float));
+  s.n = take((size_t)blocks * sizeof(int32_t));
+  s.seq = take((size_t)sequences * ((E + 31) / 32) * sizeof(double));
+  s.ticket = take(sizeof(uint32_t));
+  s.bytes = at;
+  return s;
+}
+
+template <int G, int V, int KMAX>
+static int launch_route(const RouteParams& p, int64_t blocks, cudaStream_t st) {
+  const size_t smem = (size_t)p.E * sizeof(int) + (size_t)kRouteWarps * G * V * sizeof(float);
+  route_train_kernel<G, V, KMAX><<<(unsigned)blocks, kRouteThreads, smem, st>>>(p);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+template <int G, int V>
+static int launch_route_k(const RouteParams& p, int64_t blocks, cudaStream_t st) {
+  if (p.k <= 2) return launch_route<G, V, 2>(p, blocks, st);
+  if (p.k <= 8) return launch_route<G, V, 8>(p, blocks, st);
+  return launch_route<G, V, 16>(p, blocks, st);
+}
+template <int G, int V>
+static int launch_route_bwd(const RouteBackward& p, int64_t blocks, cudaStream_t st) {
+  route_backward_kernel<G, V><<<(unsigned)blocks, kRouteThreads, 0, st>>>(p);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+static int check_route(int elem_type, int64_t ld, int64_t T, int E, int k, int64_t sequences, int scoring) {
+  if (T < 0 || E < 1 || E > kRouteMaxExperts || k < 1 || k > kRouteMaxK || k > E || T > (int64_t)0x7fffffff / k)
+    return fail(MOE_ERR_INVALID_ARG, "T=%lld E=%d k=%d (1 <= k <= min(%d, E), E <= %d, T k < 2^31)", (long long)T, E,
+                k, kRouteMaxK, kRouteMaxExperts);
+  if (sequences < 1 || sequences > (int64_t)0x7fffffff || T % sequences)
+    return fail(MOE_ERR_INVALID_ARG, "%lld tokens are not %lld sequences of equal length", (long long)T,
+                (long long)sequences);
+  if (ld < E) return fail(MOE_ERR_INVALID_ARG, "row stride %lld < E=%d", (long long)ld, E);
+  if (!elem_ok(elem_type)) return fail(MOE_ERR_UNSUPPORTED_DTYPE, "logits type %d", elem_type);
+  if (scoring != MOE_SCORE_SOFTMAX && scoring != MOE_SCORE_SIGMOID)
+    return fail(MOE_ERR_INVALID_ARG, "scoring %d (0 softmax, 1 sigmoid)", scoring);
+  return 0;
+}
+
+// Rows of whole 16-byte vectors, eight elements at a time.
+static bool route_vec(const void* base, int64_t ld, int E, int type) {
+  return E % 8 == 0 && aligned16(base) && (size_t)ld * elem_bytes(type) % 16 == 0;
+}
+
+// ------------------------------------------------------------------ rows
+// Threads per token: as few as a row has vectors for, a block where it has
+// many.
+static int row_threads(int D) { return D >= 1024 ? 256 : D >= 128 ? 32 : 8; }
+
+template <int TPT, int DY, int DYS>
+static int launch_combine(const CombineBwd& p, int zero_blocks, cudaStream_t st) {
+  combine_bwd_kernel<TPT, DY, DYS><<<(unsigned)(p.token_blocks + zero_blocks), kRowThreads, 0, st>>>(p);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+template <int TPT>
+static int launch_combine_t(CombineBwd p, int dy, int dys, int zero_blocks, cudaStream_t st) {
+  p.token_blocks = (int)((p.T + kRowThreads / TPT - 1) / (kRowThreads / TPT));
+  switch (dy * 3 + dys) {
+    case 0: return launch_combine<TPT, 0, 0>(p, zero_blocks, st);
+    case 1: return launch_combine<TPT, 0, 1>(p, zero_blocks, st);
+    case 2: return launch_combine<TPT, 0, 2>(p, zero_blocks, st);
+    case 3: return launch_combine<TPT, 1, 0>(p, zero_blocks, st);
+    case 4: return launch_combine<TPT, 1, 1>(p, zero_blocks, st);
+    case 5: return launch_combine<TPT, 1, 2>(p, zero_blocks, st);
+    case 6: return launch_combine<TPT, 2, 0>(p, zero_blocks, st);
+    case 7: return launch_combine<TPT, 2, 1>(p, zero_blocks, st);
+  }
+  return launch_combine<TPT, 2, 2>(p, zero_blocks, st);
+}
+template <int TPT, int DXS, int DX>
+static int launch_gather(const GatherBwd& p, cudaStream_t st) {
+  const int64_t blocks = (p.T + kRowThreads / TPT - 1) / (kRowThreads / TPT);
+  gather_bwd_kernel<TPT, DXS, DX><<<(unsigned)blocks, kRowThreads, 0, st>>>(p);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+template <int TPT>
+static int launch_gather_t(const GatherBwd& p, int dxs, int dx, cudaStream_t st) {
+  switch (dxs * 3 + dx) {
+    case 0: return launch_gather<TPT, 0, 0>(p, st);
+    case 1: return launch_gather<TPT, 0, 1>(p, st);
+    case 2: return launch_gather<TPT, 0, 2>(p, st);
+    case 3: return launch_gather<TPT, 1, 0>(p, st);
+    case 4: return launch_gather<TPT, 1, 1>(p, st);
+    case 5: return launch_gather<TPT, 1, 2>(p, st);
+    case 6: return launch_gather<TPT, 2, 0>(p, st);
+    case 7: return launch_gather<TPT, 2, 1>(p, st);
+  }
+  return launch_gather<TPT, 2, 2>(p, st);
+}
+
+static int check_rows(int64_t T, int k, int D, int64_t rows, int type_a, int type_b) {
+  if (T < 0 || T > 0x7fffffff || k < 1 || D <= 0 || (D & 3) || rows < 0 || rows > 0x7fffffff)
+    return fail(MOE_ERR_INVALID_ARG, "T=%lld k=%d D=%d rows=%lld (D a positive multiple of 4, T and rows < 2^31)",
+                (long long)T, k, D, (long long)rows);
+  if (!elem_ok(type_a) || !elem_ok(type_b))
+    return fail(MOE_ERR_UNSUPPORTED_DTYPE, "row types %d, %d", type_a, type_b);
+  return 0;
+}
+static bool row_aligned(const void* p, int type) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * elem_bytes(type)) == 0;
+}
+
+// ------------------------------------------------------------------ gradient lists
+static int check_tensors(const moe_tensor_desc* t, int n, int norm_type, bool with_out) {
+  if (n < 0 || (n && !t)) return fail(MOE_ERR_INVALID_ARG, "n=%d tensors=%p", n, (const void*)t);
+  if (norm_type < MOE_NORM_L1 || norm_type > MOE_NORM_INF)
+    return fail(MOE_ERR_INVALID_ARG, "norm type %d (1, 2 or 3 = infinity)", norm_type);
+  int64_t total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!elem_ok(t[i].in_type) || (with_out && !elem_ok(t[i].out_type)))
+      return fail(MOE_ERR_UNSUPPORTED_DTYPE, "tensor %d: types %d, %d", i, t[i].in_type, t[i].out_type);
+    if (t[i].rows < 0 || t[i].cols < 0 ||
+        (t[i].rows > 1 && (t[i].in_ld < t[i].cols || (with_out && t[i].out_ld < t[i].cols))))
+      return fail(MOE_ERR_INVALID_ARG, "tensor %d: %lld x %lld, strides %lld, %lld", i, (long long)t[i].rows,
+                  (long long)t[i].cols, (long long)t[i].in_ld, (long long)t[i].out_ld);
+    if (t[i].rows == 0 || t[i].cols == 0) continue;
+    constexpr int64_t kMost = (int64_t)1 << 40;  // so that units count in 32 bits
+    if (t[i].rows > kMost / t[i].cols || (total += t[i].rows * t[i].cols) > kMost)
+      return fail(MOE_ERR_UNSUPPORTED_SHAPE, "more than 2^40 elements at tensor %d", i);
+    if (!t[i].in || (with_out && !t[i].out)) return fail(MOE_ERR_INVALID_ARG, "tensor %d: null pointer", i);
+    if (reinterpret_cast<uintptr_t>(t[i].in) % elem_bytes(t[i].in_type) ||
+        (with_out && reinterpret_cast<uintptr_t>(t[i].out) % elem_bytes(t[i].out_type)))
+      return fail(MOE_ERR_MISALIGNED, "tensor %d is not aligned to its elements", i);
+  }
+  return 0;
+}
+
+static int entry_head(const GradEntry& e) {
+  const size_t in = reinterpret_cast<uintptr_t>(e.in), out = reinterpret_cast<uintptr_t>(e.out);
+  const size_t ib = elem_bytes(e.in_type), ob = elem_bytes(e.out_type);
+  if (e.rows > 1)
+    return e.cols % 8 == 0 && in % 16 == 0 && out % 16 == 0 && e.in_ld * ib % 16 == 0 && e.out_ld * ob % 16 == 0 ? 0
+                                                                                                                : -1;
+  for (int h = 0; h < 8 && h <= e.cols; ++h)
+    if ((in + h * ib) % 16 == 0 && (out + h * ob) % 16 == 0) return h;
+  return -1;
+}
+
+// Fills `list` with tensors from *at on; false when none is left.
+template <int SLOTS>
+static bool fill_list(GradList<SLOTS>& list, const moe_tensor_desc* t, int n, int* at, bool with_out) {
+  list.n = 0;
+  uint64_t units = 0;
+  for (; *at < n && list.n < SLOTS; ++*at) {
+    const moe_tensor_desc& d = t[*at];
+    if (d.rows == 0 || d.cols == 0) continue;
+    GradEntry& e = list.e[list.n];
+    e = GradEntry{d.in, with_out ? d.out : const_cast<void*>(d.in), d.rows, d.cols, d.in_ld,
+                  with_out ? d.out_ld : d.in_ld, d.in_type, with_out ? d.out_type : d.in_type, 0, (uint32_t)units};
+    e.head = entry_head(e);
+    const uint64_t more = ((uint64_t)d.rows * d.cols + kNormUnit - 1) / kNormUnit;
+    units += more;
+    ++list.n;
+  }
+  list.units = (uint32_t)units;
+  return list.n > 0;
+}
+
+static int norm_blocks(uint32_t units, int sms) {
+  return (int)std::min<int64_t>(units, std::min(kNormMaxBlocks, sms * kNormBlocksPerSm));
+}
+
+template <int NORM, int SLOTS>
+static int launch_partials(const moe_tensor_desc* t, int n, double* partial, int* count, int sms, cudaStream_t st) {
+  int at = 0;
+  *count = 0;
+  GradList<SLOTS> list;
+  while (fill_list(list, t, n, &at, false)) {
+    const int blocks = norm_blocks(list.units, sms);
+    norm_partial_kernel<NORM, SLOTS><<<blocks, kNormThreads, 0, st>>>(list, partial + *count);
+    MOE_CUDA_TRY(cudaGetLastError());
+    *count += blocks;
+  }
+  return 0;
+}
+template <int NORM, int SLOTS>
+static int launch_clip(const moe_tensor_desc* t, int n, ClipNorm c, int sms, cudaStream_t st) {
+  int at = 0;
+  GradList<SLOTS> list;
+  while (fill_list(list, t, n, &at, true)) {
+    clip_kernel<NORM, SLOTS><<<norm_blocks(list.units, sms), kNormThreads, 0, st>>>(list, c);
+    MOE_CUDA_TRY(cudaGetLastError());
+    c.norm = nullptr;
+  }
+  return 0;
+}
+template <int NORM>
+static int run_norm(const moe_tensor_desc* t, int n, float* norm, double* partial, int sms, cudaStream_t st) {
+  int count = 0;
+  const int r = n <= kGradSlotsSmall ? launch_partials<NORM, kGradSlotsSmall>(t, n, partial, &count, sms, st)
+                                     : launch_partials<NORM, kGradSlots>(t, n, partial, &count, sms, st);
+  if (r) return r;
+  norm_finish_kernel<NORM><<<1, kNormThreads, 0, st>>>(partial, count, norm);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+template <int NORM>
+static int run_clip(const moe_tensor_desc* t, int n, double max_norm, const float* given, float* norm, double* partial,
+                    int sms, cudaStream_t st) {
+  ClipNorm c{partial, 0, given, norm, max_norm};
+  const bool small = n <= kGradSlotsSmall;
+  if (!given) {
+    const int r = small ? launch_partials<NORM, kGradSlotsSmall>(t, n, partial, &c.n, sms, st)
+                        : launch_partials<NORM, kGradSlots>(t, n, partial, &c.n, sms, st);
+    if (r) return r;
+    if (c.n == 0) {  // no elements: the norm is 0 and there is nothing to scale
+      MOE_CUDA_TRY(cudaMemsetAsync(norm, 0, sizeof(float), st));
+      return 0;
+    }
+  } else if (norm && norm != given) {
+    MOE_CUDA_TRY(cudaMemcpyAsync(norm, given, sizeof(float), cudaMemcpyDeviceToDevice, st));
+  }
+  return small ? launch_clip<NORM, kGradSlotsSmall>(t, n, c, sms, st) : launch_clip<NORM, kGradSlots>(t, n, c, sms, st);
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+// ------------------------------------------------------------------ routing
+size_t moe_route_train_workspace_size(int64_t T, int32_t E, int64_t sequences) {
+  if (T < 0 || E < 1 || E > kRouteMaxExperts || sequences < 1 || T % sequences) return 0;
+  return route_space(route_chunks(T / sequences, sequences, E) * sequences, sequences, E).bytes;
+}
+
+int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
+                    int64_t sequences, const uint8_t* mask, const int32_t* given_ids, int32_t scoring,
+                    int32_t normalize, int32_t* ids, float* weights, int32_t* counts, int32_t* tokens, float* balance,
+                    float* z, void* workspace, size_t workspace_bytes, void* stream) {
+  t_err[0] = 0;
+  if (int r = check_route(elem_type, ld, T, E, k, sequences, scoring)) return r;
+  if (!counts || !tokens || !balance || !z) return fail(MOE_ERR_INVALID_ARG, "null pointer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    MOE_CUDA_TRY(cudaMemsetAsync(counts, 0, (size_t)sequences * E * sizeof(int32_t), st));
+    MOE_CUDA_TRY(cudaMemsetAsync(tokens, 0, (size_t)sequences * sizeof(int32_t), st));
+    MOE_CUDA_TRY(cudaMemsetAsync(balance, 0, sizeof(float), st));
+    MOE_CUDA_TRY(cudaMemsetAsync(z, 0, sizeof(float), st));
+    return 0;
+  }
+  if (!logits || !ids || !weights) return fail(MOE_ERR_INVALID_ARG, "null pointer");
+  if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(elem_type))
+    return fail(MOE_ERR_MISALIGNED, "logits are not aligned to their elements");
+  const int64_t seq_len = T / sequences, chunks = route_chunks(seq_len, sequences, E), blocks = chunks * sequences;
+  const RouteSpace s = route_space(blocks, sequences, E);
+  if (!workspace || workspace_bytes < s.bytes)
+    return fail(MOE_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes < required %zu", workspace_bytes, s.bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+    return fail(MOE_ERR_MISALIGNED, "workspace must be 256-byte aligned");
+  int dev;
+  DevInfo* di;
+  if (int r = device_info(&dev, &di)) return r;
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  RouteParams p{};
+  p.logits = logits;
+  p.mask = mask;
+  p.given = given_ids;
+  p.ids = ids;
+  p.weights = weights;
+  p.part_q = reinterpret_cast<float*>(w + s.q);
+  p.part_c = reinterpret_cast<int32_t*>(w + s.c);
+  p.part_z = reinterpret_cast<float*>(w + s.z);
+  p.part_n = reinterpret_cast<int32_t*>(w + s.n);
+  p.ticket = reinterpret_cast<uint32_t*>(w + s.ticket);
+  p.ld = ld;
+  p.seq_len = seq_len;
+  p.chunks = (int32_t)chunks;
+  p.E = E;
+  p.k = k;
+  p.type = elem_type;
+  p.vec = route_vec(logits, ld, E, elem_type);
+  p.sigmoid = scoring == MOE_SCORE_SIGMOID;
+  p.normalize = normalize != 0;
+  int r = 0;
+  if (E > 512) r = launch_route_k<32, 32>(p, blocks, st);
+  else if (E > 256) r = launch_route_k<32, 16>(p, blocks, st);
+  else switch (route_lanes(E)) {
+    case 1: r = launch_route_k<1, 8>(p, blocks, st); break;
+    case 2: r = launch_route_k<2, 8>(p, blocks, st); break;
+    case 4: r = launch_route_k<4, 8>(p, blocks, st); break;
+    case 8: r = launch_route_k<8, 8>(p, blocks, st); break;
+    case 16: r = launch_route_k<16, 8>(p, blocks, st); break;
+    default: r = launch_route_k<32, 8>(p, blocks, st); break;
+  }
+  if (r) return r;
+  RouteFinish f{};
+  f.part_q = p.part_q;
+  f.part_c = p.part_c;
+  f.part_z = p.part_z;
+  f.part_n = p.part_n;
+  f.ticket = p.ticket;
+  f.seq_part = reinterpret_cast<double*>(w + s.seq);
+  f.counts = counts;
+  f.tokens = tokens;
+  f.balance = balance;
+  f.z = z;
+  f.S = (int32_t)sequences;
+  f.chunks = (int32_t)chunks;
+  f.E = E;
+  f.k = k;
+  f.eblocks = (E + 31) / 32;
+  if (sequences * f.eblocks > (int64_t)0x7fffffff)
+    return fail(MOE_ERR_UNSUPPORTED_SHAPE, "%lld sequences of E=%d", (long long)sequences, E);
+  route_finish_kernel<<<(unsigned)(sequences * f.eblocks), kFinishThreads, 0, st>>>(f);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
+                       int64_t sequences, const uint8_t* mask, int32_t scoring, int32_t normalize, const int32_t* ids,
+                       const float* weights, const int32_t* counts, const int32_t* tokens, const float* d_weights,
+                       const float* d_balance, const float* d_z, void* d_logits, void* stream) {
+  t_err[0] = 0;
+  if (int r = check_route(elem_type, ld, T, E, k, sequences, scoring)) return r;
+  if (T == 0) return 0;
+  if (!logits || !ids || !weights || !counts || !tokens || !d_logits) return fail(MOE_ERR_INVALID_ARG, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(d_logits)) % elem_bytes(elem_type))
+    return fail(MOE_ERR_MISALIGNED, "logits or d_logits are not aligned to their elements");
+  int dev;
+  DevInfo* di;
+  if (int r = device_info(&dev, &di)) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  RouteBackward p{};
+  p.logits = logits;
+  p.mask = mask;
+  p.ids = ids;
+  p.weights = weights;
+  p.counts = counts;
+  p.tokens = tokens;
+  p.d_weights = d_weights;
+  p.d_balance = d_balance;
+  p.d_z = d_z;
+  p.d_logits = d_logits;
+  p.ld = ld;
+  p.seq_len = T / sequences;
+  p.chunks = (int32_t)route_chunks(p.seq_len, sequences, E);
+  p.S = (int32_t)sequences;
+  p.E = E;
+  p.k = k;
+  p.type = elem_type;
+  p.vec = route_vec(logits, ld, E, elem_type);
+  p.vec_out = route_vec(d_logits, E, E, elem_type);
+  p.sigmoid = scoring == MOE_SCORE_SIGMOID;
+  p.normalize = normalize != 0;
+  const int64_t blocks = p.chunks * sequences;
+  if (E > 512) return launch_route_bwd<32, 32>(p, blocks, st);
+  if (E > 256) return launch_route_bwd<32, 16>(p, blocks, st);
+  switch (route_lanes(E)) {
+    case 1: return launch_route_bwd<1, 8>(p, blocks, st);
+    case 2: return launch_route_bwd<2, 8>(p, blocks, st);
+    case 4: return launch_route_bwd<4, 8>(p, blocks, st);
+    case 8: return launch_route_bwd<8, 8>(p, blocks, st);
+    case 16: return launch_route_bwd<16, 8>(p, blocks, st);
+  }
+  return launch_route_bwd<32, 8>(p, blocks, st);
+}
+
+// ------------------------------------------------------------------ rows
+int moe_combine_rows_backward(const void* dy, int32_t dy_type, const float* y_sorted, const int32_t* inverse,
+                              const float* weights, const int32_t* group_sizes, int64_t T, int32_t k, int32_t D,
+                              int64_t rows, int32_t E, void* dys, int32_t dys_type, float* dw, void* stream) {
+  t_err[0] = 0;
+  if (int r = check_rows(T, k, D, rows, dy_type, dys_type)) return r;
+  if (E < 1) return fail(MOE_ERR_INVALID_ARG, "E=%d", E);
+  if (T == 0 && rows == 0) return 0;
+  if (!group_sizes || (T && (!dy || !inverse || !weights || !dw)) || (rows && (!y_sorted || !dys)))
+    return fail(MOE_ERR_INVALID_ARG, "null pointer");
+  if (!row_aligned(dy, dy_type) || !aligned16(y_sorted) || !row_aligned(dys, dys_type))
+    return fail(MOE_ERR_MISALIGNED, "rows must be aligned to 4 elements");
+  int dev;
+  DevInfo* di;
+  if (int r = device_info(&dev, &di)) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CombineBwd p{dy, y_sorted, inverse, weights, group_sizes, dys, dw, T, rows, k, D, E, 0};
+  const int zero_blocks = (int)std::min<int64_t>(di->sms, (rows * (D / 4) + kRowThreads - 1) / kRowThreads);
+  const int tpt = row_threads(D);
+  if (tpt == 256) return launch_combine_t<256>(p, dy_type, dys_type, zero_blocks, st);
+  if (tpt == 32) return launch_combine_t<32>(p, dy_type, dys_type, zero_blocks, st);
+  return launch_combine_t<8>(p, dy_type, dys_type, zero_blocks, st);
+}
+
+int moe_gather_rows_backward(const void* dxs, int32_t dxs_type, const int32_t* inverse, int64_t T, int32_t k,
+                             int32_t D, int64_t rows, void* dx, int32_t dx_type, void* stream) {
+  t_err[0] = 0;
+  if (int r = check_rows(T, k, D, rows, dxs_type, dx_type)) return r;
+  if (T == 0) return 0;
+  if (!inverse || !dx || (rows && !dxs)) return fail(MOE_ERR_INVALID_ARG, "null pointer");
+  if (!row_aligned(dxs, dxs_type) || !row_aligned(dx, dx_type))
+    return fail(MOE_ERR_MISALIGNED, "rows must be aligned to 4 elements");
+  int dev;
+  DevInfo* di;
+  if (int r = device_info(&dev, &di)) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const GatherBwd p{dxs, inverse, dx, T, rows, k, D};
+  const int tpt = row_threads(D);
+  if (tpt == 256) return launch_gather_t<256>(p, dxs_type, dx_type, st);
+  if (tpt == 32) return launch_gather_t<32>(p, dxs_type, dx_type, st);
+  return launch_gather_t<8>(p, dxs_type, dx_type, st);
+}
+
+// ------------------------------------------------------------------ gradient lists
+size_t moe_grad_norm_workspace_size(int32_t n) {
+  if (n < 0) return 0;
+  const size_t launches = (size_t)std::max(1, (n + kGradSlots - 1) / kGradSlots);
+  return align256(launches * kNormMaxBlocks * sizeof(double));
+}
+
+static int check_norm_space(int n, const void* ws, size_t bytes) {
+  const size_t need = moe_grad_norm_workspace_size(n);
+  if (!ws || bytes < need) return fail(MOE_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes < required %zu", bytes, need);
+  if (reinterpret_cast<uintptr_t>(ws) & 255u) return fail(MOE_ERR_MISALIGNED, "workspace must be 256-byte aligned");
+  return 0;
+}
+
+int moe_grad_norm(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  t_err[0] = 0;
+  if (int r = check_tensors(tensors, n, norm_type, false)) return r;
+  if (!norm) return fail(MOE_ERR_INVALID_ARG, "null norm");
+  if (int r = check_norm_space(n, workspace, workspace_bytes)) return r;
+  int dev;
+  DevInfo* di;
+  if (int r = device_info(&dev, &di)) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  if (norm_type == MOE_NORM_L1) return run_norm<kNormL1>(tensors, n, norm, partial, di->sms, st);
+  if (norm_type == MOE_NORM_L2) return run_norm<kNormL2>(tensors, n, norm, partial, di->sms, st);
+  return run_norm<kNormInf>(tensors, n, norm, partial, di->sms, st);
+}
+
+int moe_clip_grads(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type, double max_norm,
+                   const float* given_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+  t_err[0] = 0;
+  if (int r = check_tensors(tensors, n, norm_type, true)) return r;
+  if (!(max_norm >= 0.0)) return fail(MOE_ERR_INVALID_ARG, "max_norm %g", max_norm);
+  if (!given_norm && !norm) return fail(MOE_ERR_INVALID_ARG, "null norm");
+  if (!given_norm)
+    if (int r = check_norm_space(n, workspace, workspace_bytes)) return r;
+  int dev;
+  DevInfo* di;
+  if (int r = device_info(&dev, &di)) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  if (norm_type == MOE_NORM_L1) return run_clip<kNormL1>(tensors, n, max_norm, given_norm, norm, partial, di->sms, st);
+  if (norm_type == MOE_NORM_L2) return run_clip<kNormL2>(tensors, n, max_norm, given_norm, norm, partial, di->sms, st);
+  return run_clip<kNormInf>(tensors, n, max_norm, given_norm, norm, partial, di->sms, st);
+}
+
+}  // extern "C"

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/moe_b200.h"
+#include "abi_util.h"
 #include "ep_exchange.cuh"
 #include "router.cuh"
 #include "fused_pair.cuh"
@@ -22,21 +23,15 @@ namespace moe {
 __device__ int g_status = 0;
 
 // ------------------------------------------------------------------ errors
-static thread_local char t_err[512] = {0};
+thread_local char t_err[512] = {0};
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(t_err, sizeof(t_err), fmt, ap);
   va_end(ap);
   return code;
 }
-
-#define MOE_CUDA_TRY(expr)                                                                   \
-  do {                                                                                       \
-    cudaError_t _e = (expr);                                                                 \
-    if (_e != cudaSuccess) return fail(MOE_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(_e)); \
-  } while (0)
 
 // ------------------------------------------------------------------ tuning
 static int64_t g_tune_splits = 0;
@@ -196,17 +191,10 @@ static int make_map_3d(CUtensorMap* map, const void* base, CUtensorMapDataType d
 }
 
 // ------------------------------------------------------------------ device info
-struct DevInfo {
-  CUcontext ctx = nullptr;  // context the entries below belong to
-  int sms = 0;
-  int* status = nullptr;  // device address of g_status on this device
-  bool attr_set[46] = {};
-  int pairs[30] = {};  // co-resident CTA pairs per pair-kernel variant (0 = not queried)
-};
 static DevInfo g_dev[64];
 static std::mutex g_dev_mu;
 
-static int device_info(int* dev_out, DevInfo** info) {
+int device_info(int* dev_out, DevInfo** info) {
   int dev = 0;
   MOE_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(MOE_ERR_CUDA, "device ordinal %d out of range", dev);
@@ -375,7 +363,6 @@ static bool large_supported(int D, int F, int dtype) {
   if (dtype == MOE_DTYPE_F32) return D % 4 == 0 && F % 4 == 0;
   return false;
 }
-static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Large-D workspace.  bf16: H (M, F) bf16; e4m3 weights: H (M, F) f16.  f32 (3xTF32):
 // the tf32 hi/lo planes of W_up^T (E, F, D) and

@@ -22,12 +22,11 @@
 #pragma once
 #include <cstdint>
 
+#include "abi_util.h"
 #include "ptx.cuh"
 
 namespace moe {
 
-constexpr int kRouteMaxExperts = 1024;
-constexpr int kRouteMaxK = 16;
 constexpr int kPermBlock = 512;  // entries per histogram / scatter block (16 warps)
 enum : int { kStatusBadExpertId = 16 };  // an expert id outside [0, E) was dropped
 

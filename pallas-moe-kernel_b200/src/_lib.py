@@ -16,6 +16,12 @@ MOE_DTYPE_F32 = 0
 MOE_DTYPE_BF16 = 1
 MOE_DTYPE_FP8_E4M3_BLK128 = 2
 MOE_EP_HANDLE_BYTES = 256
+MOE_ELEM_F32 = 0
+MOE_ELEM_BF16 = 1
+MOE_ELEM_F16 = 2
+MOE_NORM_L1 = 1
+MOE_NORM_L2 = 2
+MOE_NORM_INF = 3
 
 ERRORS = {
     -1: "MOE_ERR_INVALID_ARG",
@@ -152,6 +158,23 @@ def lib() -> ctypes.CDLL:
     L.moe_fused_mlp_swiglu_fp8_workspace_size.restype = sz
     L.moe_fused_mlp_swiglu_fp8.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp, sz, vp]
     L.moe_fused_mlp_swiglu_fp8.restype = ctypes.c_int
+    f64 = ctypes.c_double
+    L.moe_route_train_workspace_size.argtypes = [i64, i32, i64]
+    L.moe_route_train_workspace_size.restype = sz
+    L.moe_route_train.argtypes = [vp, i32, i64, i64, i32, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.moe_route_train.restype = ctypes.c_int
+    L.moe_route_backward.argtypes = [vp, i32, i64, i64, i32, i32, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    L.moe_route_backward.restype = ctypes.c_int
+    L.moe_combine_rows_backward.argtypes = [vp, i32, vp, vp, vp, vp, i64, i32, i32, i64, i32, vp, i32, vp, vp]
+    L.moe_combine_rows_backward.restype = ctypes.c_int
+    L.moe_gather_rows_backward.argtypes = [vp, i32, vp, i64, i32, i32, i64, vp, i32, vp]
+    L.moe_gather_rows_backward.restype = ctypes.c_int
+    L.moe_grad_norm_workspace_size.argtypes = [i32]
+    L.moe_grad_norm_workspace_size.restype = sz
+    L.moe_grad_norm.argtypes = [vp, i32, i32, vp, vp, sz, vp]
+    L.moe_grad_norm.restype = ctypes.c_int
+    L.moe_clip_grads.argtypes = [vp, i32, i32, f64, vp, vp, vp, sz, vp]
+    L.moe_clip_grads.restype = ctypes.c_int
     L.moe_ep_destroy.argtypes = [vp]
     L.moe_ep_destroy.restype = ctypes.c_int
     _lib = L

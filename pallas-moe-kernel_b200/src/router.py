@@ -18,11 +18,12 @@ current stream and never synchronise the host.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
+from .kernel import _stream_handle, _stream_workspace
 
 
 def _stream(dev) -> int:
@@ -88,6 +89,204 @@ def combine_rows(y_sorted: torch.Tensor, inverse: torch.Tensor, weights: torch.T
                                            weights.float().contiguous().data_ptr(), T, k, D, out.data_ptr(),
                                            _stream(y_sorted.device)))
     return out
+
+
+# ----------------------------------------------------------------------------- training
+class RouteTrain(NamedTuple):
+    """Result of :func:`route_forward_train`."""
+    ids: torch.Tensor           # (T, k) int32, -1: no expert
+    weights: torch.Tensor       # (T, k) f32
+    counts: torch.Tensor        # (sequences, E) int32: chosen entries per expert
+    tokens: torch.Tensor        # (sequences,) int32: tokens that take part
+    balance_loss: torch.Tensor  # f32 scalar
+    z_loss: torch.Tensor        # f32 scalar
+
+
+_ELEMS = {torch.float32: _lib.MOE_ELEM_F32, torch.bfloat16: _lib.MOE_ELEM_BF16, torch.float16: _lib.MOE_ELEM_F16}
+_SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def _elem(t: torch.Tensor, name: str) -> int:
+    code = _ELEMS.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} is {t.dtype} (float32, bfloat16 or float16)")
+    return code
+
+
+def _on(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the other operands on {dev}")
+
+
+def _call(dev: torch.device, fn, *args) -> None:
+    """One library call on ``dev`` and its current stream."""
+    if dev.index == torch.cuda.current_device():
+        _lib.check(fn(*args, _stream_handle(dev)))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, _stream_handle(dev)))
+
+
+def _route_args(logits, mask, sequences, scoring):
+    """(logits with unit column stride, element type, row stride, mask bytes, scoring code)."""
+    if not logits.is_cuda or logits.dim() != 2:
+        raise ValueError("logits must be a 2-D CUDA tensor")
+    code = _elem(logits, "logits")
+    T, E = logits.shape
+    if E > 1 and logits.stride(1) != 1 or T > 1 and logits.stride(0) < E:
+        logits = logits.contiguous()
+    if sequences < 1 or T % sequences:
+        raise ValueError(f"{T} tokens are not {sequences} sequences of equal length")
+    how = _SCORING.get(scoring)
+    if how is None:
+        raise ValueError(f"scoring {scoring!r} is not 'softmax' or 'sigmoid'")
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.numel() != T:
+            raise ValueError(f"mask must be a bool tensor with one value per token ({T})")
+        _on(logits.device, mask=mask)
+        mask = mask.contiguous()
+    return logits, code, logits.stride(0) if T > 1 else E, mask, how
+
+
+def route_forward_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Tensor] = None,
+                        mask: Optional[torch.Tensor] = None, sequences: int = 1, scoring: str = "softmax",
+                        normalize: bool = True, workspace: Optional[torch.Tensor] = None) -> RouteTrain:
+    """Top-k routing with the balance and z losses and per-expert counts.
+
+    ``logits`` (T, E) float32, bfloat16 or float16; the T tokens are
+    ``sequences`` runs of equal length.  Per token, with p = softmax(logits),
+    s = sigmoid(logits) and q = p (``scoring="softmax"``) or s / sum(s)
+    (``"sigmoid"``): the k largest logits (ties to the lower expert id) and
+    their scores p or s, divided by their sum with ``normalize``;
+
+        balance_loss = mean over sequences of sum_e (c_e E / (k N)) mean_t(q_te)
+        z_loss       = mean over tokens of logsumexp(logits)^2
+
+    with c_e the entries that chose expert e in a sequence of N tokens.
+    ``mask`` (T,) bool: tokens where it is False (padding) take no part - ids
+    -1, weights 0 - and neither does a token whose logits are all -inf.  An
+    expert whose logit is -inf is never chosen; its slots get id -1.  ``ids``
+    (T, k): experts chosen elsewhere, to be used in place of the top k.
+
+    ``permute`` drops the -1 entries and reports them in the device status
+    word.  The gradient is :func:`route_backward`; ``train.route_topk_train``
+    puts both under autograd."""
+    logits, code, ld, mask, how = _route_args(logits, mask, sequences, scoring)
+    dev = logits.device
+    T, E = logits.shape
+    if ids is not None:
+        if tuple(ids.shape) != (T, k):
+            raise ValueError(f"ids is {tuple(ids.shape)}, expected {(T, k)}")
+        _on(dev, ids=ids)
+        ids = ids.to(torch.int32).contiguous()
+    if not 1 <= k <= min(16, E) or E > 1024:
+        raise ValueError(f"k={k}, E={E}: 1 <= k <= min(16, E) and E <= 1024 are supported")
+    i32 = {"dtype": torch.int32, "device": dev}
+    f32 = {"dtype": torch.float32, "device": dev}
+    out = RouteTrain(torch.empty((T, k), **i32), torch.empty((T, k), **f32), torch.empty((sequences, E), **i32),
+                     torch.empty(sequences, **i32), torch.empty((), **f32), torch.empty((), **f32))
+    L = _lib.lib()
+    need = int(L.moe_route_train_workspace_size(T, E, sequences))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = _stream_workspace(dev, _stream_handle(dev), need)
+    _call(dev, L.moe_route_train, logits.data_ptr(), code, ld, T, E, k, sequences,
+          None if mask is None else mask.data_ptr(), None if ids is None else ids.data_ptr(), how, normalize,
+          *(t.data_ptr() for t in out), workspace.data_ptr(), need)
+    return out
+
+
+def route_backward(logits: torch.Tensor, routed: RouteTrain, *, d_weights: Optional[torch.Tensor] = None,
+                   d_balance: Optional[torch.Tensor] = None, d_z: Optional[torch.Tensor] = None,
+                   mask: Optional[torch.Tensor] = None, sequences: int = 1, scoring: str = "softmax",
+                   normalize: bool = True) -> torch.Tensor:
+    """Gradient (T, E) with respect to the logits, in their type, for upstream
+    gradients of the weights (T, k) and of the two losses (scalars on the
+    device); a gradient that is None counts as zero.  ``routed`` is the
+    forward's result for the same logits and options."""
+    logits, code, ld, mask, how = _route_args(logits, mask, sequences, scoring)
+    dev = logits.device
+    T, E = logits.shape
+    k = routed.ids.shape[1]
+    if tuple(routed.ids.shape) != (T, k) or tuple(routed.counts.shape) != (sequences, E):
+        raise ValueError(f"routed has ids {tuple(routed.ids.shape)} and counts {tuple(routed.counts.shape)}, "
+                         f"expected {(T, k)} and {(sequences, E)}")
+    if d_weights is not None:
+        if tuple(d_weights.shape) != (T, k):
+            raise ValueError(f"d_weights is {tuple(d_weights.shape)}, expected {(T, k)}")
+        d_weights = d_weights.to(torch.float32).contiguous()
+    for name, g in (("d_balance", d_balance), ("d_z", d_z)):
+        if g is not None and (g.numel() != 1 or g.dtype != torch.float32):
+            raise ValueError(f"{name} must be a float32 scalar tensor")
+    _on(dev, ids=routed.ids, d_weights=d_weights, d_balance=d_balance, d_z=d_z)
+    d = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _call(dev, _lib.lib().moe_route_backward, logits.data_ptr(), code, ld, T, E, k, sequences, ptr(mask), how,
+          normalize, routed.ids.data_ptr(), routed.weights.data_ptr(), routed.counts.data_ptr(),
+          routed.tokens.data_ptr(), ptr(d_weights), ptr(d_balance), ptr(d_z), d.data_ptr())
+    return d
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    if not t.is_cuda or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D CUDA tensor")
+    if t.shape[1] % 4 or t.shape[1] == 0:
+        raise ValueError(f"{name} has rows of {t.shape[1]} elements: a positive multiple of 4 is needed")
+    t = t.contiguous()
+    # A contiguous view may start anywhere in its storage; the kernels read
+    # four elements at a time.
+    return t if t.data_ptr() % (4 * t.element_size()) == 0 else t.clone()
+
+
+def combine_rows_backward(dy: torch.Tensor, y_sorted: torch.Tensor, inverse: torch.Tensor, weights: torch.Tensor,
+                          group_sizes: torch.Tensor, *, dtype: torch.dtype = torch.float32
+                          ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Backward of :func:`combine_rows` for the upstream gradient ``dy``
+    (T, D): (dys, dw) with ``dys[inverse[t, j]] = weights[t, j] * dy[t]`` in
+    ``dtype`` - rows past ``sum(group_sizes)`` zero - and the f32 weights'
+    gradient ``dw[t, j] = <dy[t], y_sorted[inverse[t, j]]>``, 0 at dropped
+    entries.  bfloat16 ``dys`` are what the experts' backward multiplies."""
+    code = _elem(dy, "dy")
+    dy, y_sorted = _rows(dy, "dy"), _rows(y_sorted, "y_sorted")
+    dev = dy.device
+    T, k = inverse.shape
+    N, D = y_sorted.shape
+    if tuple(dy.shape) != (T, D) or tuple(weights.shape) != (T, k):
+        raise ValueError(f"dy {tuple(dy.shape)}, weights {tuple(weights.shape)}: expected {(T, D)} and {(T, k)}")
+    if y_sorted.dtype != torch.float32 or inverse.dtype != torch.int32:
+        raise TypeError("y_sorted must be float32 and inverse int32")
+    if dtype not in _ELEMS:
+        raise TypeError(f"dtype {dtype} (float32, bfloat16 or float16)")
+    _on(dev, y_sorted=y_sorted, inverse=inverse, weights=weights, group_sizes=group_sizes)
+    inverse, weights = inverse.contiguous(), weights.to(torch.float32).contiguous()
+    gs = group_sizes.to(torch.int32).contiguous()
+    dys = torch.empty((N, D), dtype=dtype, device=dev)
+    dw = torch.empty((T, k), dtype=torch.float32, device=dev)
+    _call(dev, _lib.lib().moe_combine_rows_backward, dy.data_ptr(), code, y_sorted.data_ptr(), inverse.data_ptr(),
+          weights.data_ptr(), gs.data_ptr(), T, k, D, N, gs.numel(), dys.data_ptr(), _ELEMS[dtype], dw.data_ptr())
+    return dys, dw
+
+
+def gather_rows_backward(dxs: torch.Tensor, inverse: torch.Tensor, *, dtype: Optional[torch.dtype] = None
+                         ) -> torch.Tensor:
+    """Backward of :func:`gather_rows`: ``dx[t] = sum_j dxs[inverse[t, j]]``,
+    summed in f32 in slot order, in ``dtype`` (default: ``dxs``'s)."""
+    code = _elem(dxs, "dxs")
+    dxs = _rows(dxs, "dxs")
+    dev = dxs.device
+    T, k = inverse.shape
+    N, D = dxs.shape
+    dtype = dxs.dtype if dtype is None else dtype
+    if inverse.dtype != torch.int32:
+        raise TypeError("inverse must be int32")
+    if dtype not in _ELEMS:
+        raise TypeError(f"dtype {dtype} (float32, bfloat16 or float16)")
+    _on(dev, inverse=inverse)
+    inverse = inverse.contiguous()
+    dx = torch.empty((T, D), dtype=dtype, device=dev)
+    _call(dev, _lib.lib().moe_gather_rows_backward, dxs.data_ptr(), code, inverse.data_ptr(), T, k, D, N,
+          dx.data_ptr(), _ELEMS[dtype])
+    return dx
 
 
 def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, k: int, *,

@@ -23,10 +23,12 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
+from . import router
 from .kernel import _as_device_group_sizes
 
 __all__ = ["forward_train", "backward", "FusedRaggedMLP", "fused_ragged_mlp_train", "swiglu_forward_train",
-           "swiglu_backward", "FusedRaggedSwiGLU", "fused_ragged_swiglu_train"]
+           "swiglu_backward", "FusedRaggedSwiGLU", "fused_ragged_swiglu_train", "RouteTopK", "route_topk_train",
+           "RoutedExperts", "moe_layer_train"]
 
 
 def _vp(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -231,3 +233,87 @@ def fused_ragged_swiglu_train(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: 
     """Differentiable SwiGLU experts: ``ragged_dot(silu(X W_gate) * (X W_up), W_down)``
     with ``w_gate_up = swiglu_interleave(w_gate, w_up)``."""
     return FusedRaggedSwiGLU.apply(x, w_gate_up, w_down, group_sizes)
+
+
+# ----------------------------------------------------------------------------- a whole layer
+class RouteTopK(torch.autograd.Function):
+    """Autograd node of ``router.route_forward_train``: gradients of the
+    weights, the balance loss and the z loss reach the logits in one pass."""
+
+    @staticmethod
+    def forward(ctx, logits, k, ids, mask, sequences, scoring, normalize):
+        r = router.route_forward_train(logits, k, ids=ids, mask=mask, sequences=sequences, scoring=scoring,
+                                       normalize=normalize)
+        ctx.options = {"sequences": sequences, "scoring": scoring, "normalize": normalize}
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(r.ids, r.counts, r.tokens)
+        ctx.save_for_backward(logits, mask, r.ids, r.weights, r.counts, r.tokens)
+        return tuple(r)
+
+    @staticmethod
+    def backward(ctx, _ids, dw, _counts, _tokens, d_balance, d_z):
+        logits, mask, ids, weights, counts, tokens = ctx.saved_tensors
+        if dw is None and d_balance is None and d_z is None:
+            return (None,) * 7
+        routed = router.RouteTrain(ids, weights, counts, tokens, None, None)
+        d = router.route_backward(logits, routed, d_weights=dw, d_balance=d_balance, d_z=d_z, mask=mask, **ctx.options)
+        return (d,) + (None,) * 6
+
+
+def route_topk_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Tensor] = None,
+                     mask: Optional[torch.Tensor] = None, sequences: int = 1, scoring: str = "softmax",
+                     normalize: bool = True) -> router.RouteTrain:
+    """Differentiable ``router.route_forward_train`` (same arguments): weights,
+    balance loss and z loss carry gradients to the logits."""
+    return router.RouteTrain(*RouteTopK.apply(logits, k, ids, mask, sequences, scoring, normalize))
+
+
+class RoutedExperts(torch.autograd.Function):
+    """Autograd node of permute -> gather -> experts -> weighted combine: y
+    (T, D) f32 from token rows, routing weights and expert weights.  One node,
+    so that the gradient of the expert outputs goes to the experts' backward in
+    the bf16 that its products take and never exists in f32."""
+
+    @staticmethod
+    def forward(ctx, x, weights, w_in, w_down, ids, swiglu):
+        gs, src, inv = router.permute(ids, w_in.shape[0])
+        xs = router.gather_rows(x, src, ids.shape[1])
+        ys, saved = (swiglu_forward_train if swiglu else forward_train)(xs, w_in, w_down, gs)
+        ctx.swiglu = swiglu
+        ctx.save_for_backward(xs, weights, w_in, w_down, gs, inv, ys, saved)
+        return router.combine_rows(ys, inv, weights)
+
+    @staticmethod
+    def backward(ctx, dy):
+        xs, weights, w_in, w_down, gs, inv, ys, saved = ctx.saved_tensors
+        dys, dw = router.combine_rows_backward(dy, ys, inv, weights, gs, dtype=torch.bfloat16)
+        dxs, dw_in, dw_down = (swiglu_backward if ctx.swiglu else backward)(xs, w_in, w_down, gs, saved, dys)
+        dx = router.gather_rows_backward(dxs, inv, dtype=xs.dtype)
+        return dx, dw, dw_in.to(w_in.dtype), dw_down.to(w_down.dtype), None, None
+
+
+def moe_layer_train(x: torch.Tensor, logits: torch.Tensor, w_in: torch.Tensor, w_down: torch.Tensor, k: int, *,
+                    activation: str = "gelu", mask: Optional[torch.Tensor] = None, sequences: int = 1,
+                    scoring: str = "softmax", normalize: bool = True) -> Tuple[torch.Tensor, router.RouteTrain]:
+    """Differentiable MoE layer: top-k routing of ``x`` (T, D) bf16 by
+    ``logits`` (T, E), the experts over the expert-sorted rows and the weighted
+    combine.  Returns (y (T, D) f32, routed) with ``routed.balance_loss`` and
+    ``routed.z_loss`` to be added to the loss:
+
+        y, routed = moe_layer_train(x, x @ w_router, w_up, w_down, k=2)
+        (loss(y) + 0.01 * routed.balance_loss + 0.001 * routed.z_loss).backward()
+
+    ``w_in`` is w_up (E, D, F) with ``activation="gelu"``, or the interleaved
+    gate/up weights (E, D, 2F) of ``swiglu_interleave`` with ``"swiglu"``; the
+    routing options are those of ``router.route_forward_train`` (padded tokens,
+    which ``mask`` leaves out, get y = 0 and no gradient).  D and F multiples
+    of 256, as for the experts' training entry points."""
+    if activation not in ("gelu", "swiglu"):
+        raise ValueError(f"activation {activation!r} is not 'gelu' or 'swiglu'")
+    M, D, F, E = (_check_swiglu if activation == "swiglu" else _check)(x, w_in, w_down)
+    if tuple(logits.shape) != (M, E) or logits.device != x.device:
+        raise ValueError(f"logits {tuple(logits.shape)} on {logits.device}: expected {(M, E)} on {x.device}")
+    with torch.cuda.device(x.device):
+        routed = route_topk_train(logits, k, mask=mask, sequences=sequences, scoring=scoring, normalize=normalize)
+        y = RoutedExperts.apply(x, routed.weights, w_in, w_down, routed.ids, activation == "swiglu")
+    return y, routed
