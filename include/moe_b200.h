@@ -429,7 +429,10 @@ enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
  * top k (an id outside [0, E) counts as -1; one id may come up twice).
  * E <= 1024, k <= min(16, E), T k < 2^31.  A NaN logit of a token that takes
  * part makes the losses NaN.  Workspace: moe_route_train_workspace_size
- * bytes, 256-byte aligned.
+ * bytes, 256-byte aligned.  counters: moe_route_train_counters uint32 of
+ * device memory that are zero at the first call which gets them; every call
+ * leaves them zero.  Calls that may overlap need workspaces and counters of
+ * their own.
  *
  * moe_route_backward: d_logits (T, E) contiguous, of elem_type, for the
  * upstream gradients d_weights (T, k) f32, d_balance and d_z (device f32
@@ -438,10 +441,11 @@ enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
  * Tokens that take no part, and logits of -inf, get 0.
  */
 size_t moe_route_train_workspace_size(int64_t T, int32_t E, int64_t sequences);
+int64_t moe_route_train_counters(int64_t T, int32_t E, int64_t sequences);
 int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
                     int64_t sequences, const uint8_t* mask, const int32_t* given_ids, int32_t scoring,
                     int32_t normalize, int32_t* ids, float* weights, int32_t* counts, int32_t* tokens, float* balance,
-                    float* z, void* workspace, size_t workspace_bytes, void* stream);
+                    float* z, void* workspace, size_t workspace_bytes, uint32_t* counters, void* stream);
 int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
                        int64_t sequences, const uint8_t* mask, int32_t scoring, int32_t normalize, const int32_t* ids,
                        const float* weights, const int32_t* counts, const int32_t* tokens, const float* d_weights,

@@ -1,12 +1,13 @@
 // Global norm of a list of tensors, and their scaling to a largest norm
 // (sm_100a).
 //
-//   norm_partial_kernel  each block walks units of kNormUnit elements over all
-//                        tensors and writes one f64 partial;
+//   norm_partial_kernel  each block walks units of 32 KB over all tensors and
+//                        writes one f64 partial;
 //   norm_finish_kernel   one block adds the partials in order: the norm (f32);
 //   clip_kernel          out = in * min(1, max_norm / (norm + 1e-6)), rounded
 //                        once to out's type; its blocks add the partials
-//                        themselves, which saves the finish launch.
+//                        themselves, which saves the finish launch.  One
+//                        launch per pair of types in the list.
 //
 // HBM-bound: the tensors are read once for the norm and once for the scaling
 // (from L2 where they fit: the scaling walks the units backwards, so that it
@@ -29,22 +30,25 @@
 namespace moe {
 
 constexpr int kNormThreads = 256;
-constexpr int kNormVecs = 4;                                // 8-element vectors a thread takes per unit
-constexpr int kNormUnit = kNormThreads * kNormVecs * 8;     // elements
+constexpr int kNormChunks = 8;                          // 16-byte chunks of input a thread has in flight
 constexpr int kNormBlocksPerSm = 4;
-constexpr int kNormMaxBlocks = 148 * kNormBlocksPerSm;      // most blocks (partials) of one launch
+constexpr int kNormMaxBlocks = 148 * kNormBlocksPerSm;  // most blocks (partials) of one launch
+
+// Elements of a chunk and of a unit (32 KB of input).
+__host__ __device__ constexpr int chunk_elems(int type) { return type == kElemF32 ? 4 : 8; }
+__host__ __device__ constexpr int64_t unit_elems(int type) { return kNormThreads * kNormChunks * chunk_elems(type); }
 
 // rows x cols elements, rows in_ld / out_ld elements apart (a dense tensor is
 // one row).  head: elements before the first one that is 16-byte aligned in
-// `in` and in `out` (0 for every tensor of several rows); -1: no such element,
-// the tensor is read one element at a time.
+// `in` and in `out` aligned to the store of a chunk (0 for every tensor of
+// several rows); -1: no such element, the tensor is read one element at a
+// time.
 struct GradEntry {
   const void* in;
   void* out;
   int64_t rows, cols, in_ld, out_ld;
-  int32_t in_type, out_type;
-  int32_t head;
-  uint32_t unit0;  // first unit of this tensor in its launch
+  int16_t in_type, out_type;
+  int16_t head;
 };
 
 constexpr int kGradSlotsSmall = 48;   // launch arguments of 3 KB
@@ -52,23 +56,13 @@ constexpr int kGradSlots = 500;       // 32 KB (the most that a launch takes is 
 template <int SLOTS>
 struct GradList {
   GradEntry e[SLOTS];
+  uint32_t unit0[SLOTS];  // first unit of each tensor; apart from the entries, so that a search reads few lines
   int32_t n;
   uint32_t units;
 };
+static_assert(sizeof(GradList<kGradSlots>) < 32000, "launch arguments end at 32,764 bytes");
 
 enum : int { kNormL1 = 1, kNormL2 = 2, kNormInf = 3 };
-
-// The entry of a unit: the last one whose first unit is not past it.
-template <int SLOTS>
-__device__ __forceinline__ int entry_of(const GradList<SLOTS>& list, uint32_t unit) {
-  int lo = 0, hi = list.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (list.e[mid].unit0 <= unit) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
 
 // Element i of the tensor (row-major over rows x cols) as an offset.
 __device__ __forceinline__ int64_t entry_at(int64_t i, int64_t rows, int64_t cols, int64_t ld) {
@@ -77,24 +71,65 @@ __device__ __forceinline__ int64_t entry_at(int64_t i, int64_t rows, int64_t col
   return r * ld + (i - r * cols);
 }
 
-// A block's pass over one unit: f8(in offset, out offset) per vector of 8 and
-// f1(...) per single element.  The first unit of a tensor also takes the
-// elements before and after the vectors.
-template <class F8, class F1>
-__device__ __forceinline__ void walk_unit(const GradEntry& e, int64_t u, F8&& f8, F1&& f1) {
-  const int64_t total = e.rows * e.cols, rows = e.rows, cols = e.cols;
+// The 16-bit and f32 types' values of a chunk.
+template <int TYPE>
+__device__ __forceinline__ void chunk_values(const uint4& r, float* v) {
+  if (TYPE == kElemF32) {
+    v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
+  } else {
+    unpack16(r.x, TYPE, v[0], v[1]);
+    unpack16(r.y, TYPE, v[2], v[3]);
+    unpack16(r.z, TYPE, v[4], v[5]);
+    unpack16(r.w, TYPE, v[6], v[7]);
+  }
+}
+// Plain loads throughout: the scaling may run in place, and the read-only
+// path is for memory that nobody writes during the kernel.
+template <int TYPE>
+__device__ __forceinline__ float single_value(const void* p, int64_t i) {
+  if (TYPE == kElemF32) return static_cast<const float*>(p)[i];
+  const uint16_t u = static_cast<const uint16_t*>(p)[i];
+  return TYPE == kElemBF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+}
+template <int TYPE>
+__device__ __forceinline__ const uint4* chunk_ptr(const void* p, int64_t i) {
+  return reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (TYPE == kElemF32 ? 4 : 2));
+}
+
+// A block's pass over one unit: all of a thread's chunks are loaded, then
+// chunks(raw, index of the first, number in the tensor) takes them (zeros past
+// the end); single(in offset, out offset) takes the elements outside chunks:
+// those before and after (in a tensor's first unit), or all where head < 0.
+template <int TYPE, class Chunks, class Single>
+__device__ __forceinline__ void walk_unit(const GradEntry& e, int64_t u, Chunks&& chunks, Single&& single) {
+  constexpr int CE = chunk_elems(TYPE);
+  const int64_t rows = e.rows, cols = e.cols, total = rows * cols;
   if (e.head < 0) {
-    const int64_t hi = min(total, (u + 1) * kNormUnit);
-    for (int64_t i = u * kNormUnit + threadIdx.x; i < hi; i += kNormThreads)
-      f1(entry_at(i, rows, cols, e.in_ld), entry_at(i, rows, cols, e.out_ld));
+    const int64_t hi = min(total, (u + 1) * unit_elems(TYPE));
+    for (int64_t i = u * unit_elems(TYPE) + threadIdx.x; i < hi; i += kNormThreads)
+      single(entry_at(i, rows, cols, e.in_ld), entry_at(i, rows, cols, e.out_ld));
     return;
   }
-  const int64_t nvec = (total - e.head) >> 3;
-  f8(u * (kNormUnit / 8) + threadIdx.x, nvec);
+  const int64_t n = (total - e.head) / CE;  // chunks
+  const int64_t first = u * (kNormThreads * kNormChunks) + threadIdx.x;
+  uint4 raw[kNormChunks];
+  if (rows == 1) {
+    const uint4* q = chunk_ptr<TYPE>(e.in, e.head) + first;
+#pragma unroll
+    for (int s = 0; s < kNormChunks; ++s)
+      raw[s] = first + s * kNormThreads < n ? q[s * kNormThreads] : make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int s = 0; s < kNormChunks; ++s)
+      raw[s] = first + s * kNormThreads < n
+                   ? *chunk_ptr<TYPE>(e.in, entry_at((first + s * kNormThreads) * CE, rows, cols, e.in_ld))
+                   : make_uint4(0, 0, 0, 0);
+  }
+  chunks(raw, first, n);
   if (u == 0) {
-    const int64_t tail = e.head + 8 * nvec;
-    int64_t i = threadIdx.x < 8 ? threadIdx.x : tail + threadIdx.x - 8;
-    if (threadIdx.x < 8 ? i < e.head : threadIdx.x < 16 && i < total) f1(i, i);
+    const int64_t tail = e.head + CE * n;
+    const int64_t i = threadIdx.x < 8 ? (int64_t)threadIdx.x : tail + threadIdx.x - 8;
+    if (threadIdx.x < 8 ? i < e.head : threadIdx.x < 16 && i < total) single(i, i);
   }
 }
 
@@ -135,36 +170,34 @@ __device__ __forceinline__ void norm_add(const float (&v)[N], NormAcc& acc) {
 
 template <int NORM, int TYPE>
 __device__ __forceinline__ void norm_unit(const GradEntry& e, int64_t u, NormAcc& acc) {
-  walk_unit(
+  constexpr int CE = chunk_elems(TYPE), PER = 32 / CE;  // chunks of 32 elements
+  walk_unit<TYPE>(
       e, u,
-      [&](int64_t first, int64_t nvec) {
-        float v[kNormVecs * 8];
+      [&](const uint4 (&raw)[kNormChunks], int64_t, int64_t) {
 #pragma unroll
-        for (int s = 0; s < kNormVecs; ++s) {
-          const int64_t i = first + s * kNormThreads;
-          if (i < nvec) {
-            elem_load8(e.in, TYPE, entry_at(e.head + 8 * i, e.rows, e.cols, e.in_ld), v + 8 * s);
-          } else {
+        for (int s = 0; s < kNormChunks; s += PER) {
+          float v[32];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) v[8 * s + x] = 0.f;
-          }
+          for (int c = 0; c < PER; ++c) chunk_values<TYPE>(raw[s + c], v + c * CE);
+          norm_add<NORM>(v, acc);
         }
-        norm_add<NORM>(v, acc);
       },
       [&](int64_t in, int64_t) {
-        const float v[1] = {elem_load(e.in, TYPE, in)};
+        const float v[1] = {single_value<TYPE>(e.in, in)};
         norm_add<NORM>(v, acc);
       });
 }
 
 template <int NORM, int SLOTS>
-__global__ void __launch_bounds__(kNormThreads) norm_partial_kernel(const __grid_constant__ GradList<SLOTS> list,
+__global__ void __launch_bounds__(kNormThreads, kNormBlocksPerSm) norm_partial_kernel(const __grid_constant__ GradList<SLOTS> list,
                                                                     double* __restrict__ partial) {
   __shared__ double s_w[kNormThreads / 32];
   NormAcc acc{0.0, 0u};
+  int at = 0;
   for (uint32_t unit = blockIdx.x; unit < list.units; unit += gridDim.x) {
-    const GradEntry& e = list.e[entry_of(list, unit)];
-    const int64_t u = unit - e.unit0;
+    while (at + 1 < list.n && list.unit0[at + 1] <= unit) ++at;
+    const GradEntry& e = list.e[at];
+    const int64_t u = unit - list.unit0[at];
     if (e.in_type == kElemF32) norm_unit<NORM, kElemF32>(e, u, acc);
     else if (e.in_type == kElemBF16) norm_unit<NORM, kElemBF16>(e, u, acc);
     else norm_unit<NORM, kElemF16>(e, u, acc);
@@ -185,113 +218,95 @@ __global__ void __launch_bounds__(kNormThreads) norm_partial_kernel(const __grid
 }
 
 // The norm from n partials, the same value in every thread of the block.
-template <int NORM>
-__device__ __forceinline__ float norm_of(const double* partial, int n, double* s_w) {
+__device__ __forceinline__ float norm_of(int norm_type, const double* partial, int n, double* s_w) {
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) v = NORM == kNormInf ? fmax(v, partial[i]) : v + partial[i];
-  if (NORM == kNormInf) {
+  if (norm_type == kNormInf) {
+    for (int i = threadIdx.x; i < n; i += kNormThreads) v = fmax(v, partial[i]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
     if ((threadIdx.x & 31) == 0) s_w[threadIdx.x >> 5] = v;
     __syncthreads();
-    for (int w = 0; w < (int)blockDim.x >> 5; ++w) v = fmax(v, s_w[w]);
+    for (int w = 0; w < kNormThreads / 32; ++w) v = fmax(v, s_w[w]);
     return __uint_as_float((uint32_t)v);  // the bits of |x|: whole numbers below 2^32
   }
+  for (int i = threadIdx.x; i < n; i += kNormThreads) v += partial[i];
   v = block_sum(v, s_w);
-  return (float)(NORM == kNormL2 ? sqrt(v) : v);
+  return (float)(norm_type == kNormL2 ? sqrt(v) : v);
 }
 
-template <int NORM>
-__global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(const double* partial, int n, float* norm) {
+__global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(int norm_type, const double* partial, int n,
+                                                                   float* norm) {
   __shared__ double s_w[kNormThreads / 32];
-  const float v = norm_of<NORM>(partial, n, s_w);
+  const float v = norm_of(norm_type, partial, n, s_w);
   if (threadIdx.x == 0) *norm = v;
 }
 
 // ---------------------------------------------------------------- clip
-// in may be out: plain loads (the read-only path is for memory that nobody
-// writes during the kernel).
-template <int TYPE>
-__device__ __forceinline__ void clip_load8(const void* p, int64_t i, float* v) {
-  if (TYPE == kElemF32) {
-    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const float4 a = q[0], b = q[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-    unpack16(a.x, TYPE, v[0], v[1]);
-    unpack16(a.y, TYPE, v[2], v[3]);
-    unpack16(a.z, TYPE, v[4], v[5]);
-    unpack16(a.w, TYPE, v[6], v[7]);
-  }
-}
-template <int TYPE>
-__device__ __forceinline__ float clip_load(const void* p, int64_t i) {
-  if (TYPE == kElemF32) return static_cast<const float*>(p)[i];
-  const uint16_t u = static_cast<const uint16_t*>(p)[i];
-  return TYPE == kElemBF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
-}
-
 template <int IN, int OUT>
 __device__ __forceinline__ void clip_unit(const GradEntry& e, int64_t u, float coef) {
-  walk_unit(
+  constexpr int CE = chunk_elems(IN);
+  const int64_t rows = e.rows;
+  walk_unit<IN>(
       e, u,
-      [&](int64_t first, int64_t nvec) {
-        float v[kNormVecs * 8];
+      [&](const uint4 (&raw)[kNormChunks], int64_t first, int64_t n) {
 #pragma unroll
-        for (int s = 0; s < kNormVecs; ++s) {
-          const int64_t i = first + s * kNormThreads;
-          if (i < nvec) clip_load8<IN>(e.in, entry_at(e.head + 8 * i, e.rows, e.cols, e.in_ld), v + 8 * s);
-        }
+        for (int s = 0; s < kNormChunks; ++s) {
+          const int64_t c = first + s * kNormThreads;
+          if (c >= n) continue;
+          float v[CE];
+          chunk_values<IN>(raw[s], v);
 #pragma unroll
-        for (int s = 0; s < kNormVecs; ++s) {
-          const int64_t i = first + s * kNormThreads;
-          if (i >= nvec) continue;
+          for (int x = 0; x < CE; ++x) v[x] *= coef;
+          const int64_t at = rows == 1 ? e.head + c * CE : entry_at(c * CE, rows, e.cols, e.out_ld);
+          if (OUT == kElemF32) {
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[8 * s + x] *= coef;
-          elem_store8(e.out, OUT, entry_at(e.head + 8 * i, e.rows, e.cols, e.out_ld), v + 8 * s);
+            for (int x = 0; x < CE; x += 4)
+              *reinterpret_cast<float4*>(static_cast<float*>(e.out) + at + x) =
+                  make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          } else if (CE == 4) {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(e.out) + at) =
+                make_uint2(pack16(v[0], v[1], OUT), pack16(v[2], v[3], OUT));
+          } else {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(e.out) + at) =
+                make_uint4(pack16(v[0], v[1], OUT), pack16(v[2], v[3], OUT), pack16(v[4 % CE], v[5 % CE], OUT),
+                           pack16(v[6 % CE], v[7 % CE], OUT));
+          }
         }
       },
-      [&](int64_t in, int64_t out) { elem_store(e.out, OUT, out, clip_load<IN>(e.in, in) * coef); });
+      [&](int64_t in, int64_t out) { elem_store(e.out, OUT, out, single_value<IN>(e.in, in) * coef); });
 }
 
 struct ClipNorm {
   const double* partial;  // n partials of the norm, or
   int32_t n;
+  int32_t norm_type;
   const float* given;     // the norm itself
   float* norm;            // written by block 0 from the partials
   double max_norm;
 };
 
-template <int NORM, int SLOTS>
-__global__ void __launch_bounds__(kNormThreads) clip_kernel(const __grid_constant__ GradList<SLOTS> list,
+// One pair of types per launch: a switch over all pairs around this body
+// spilled 2 KB a thread and ran the 2 x 470 M element case at 1625 us.
+template <int IN, int OUT, int SLOTS>
+__global__ void __launch_bounds__(kNormThreads, kNormBlocksPerSm) clip_kernel(const __grid_constant__ GradList<SLOTS> list,
                                                             const ClipNorm c) {
   __shared__ double s_w[kNormThreads / 32];
   float norm;
   if (c.given) {
     norm = *c.given;
   } else {
-    norm = norm_of<NORM>(c.partial, c.n, s_w);
+    norm = norm_of(c.norm_type, c.partial, c.n, s_w);
     if (c.norm && blockIdx.x == 0 && threadIdx.x == 0) *c.norm = norm;
   }
   const double ratio = c.max_norm / ((double)norm + 1e-6);
-  const float coef = ratio < 1.0 ? (float)ratio : ratio >= 1.0 ? 1.f : (float)ratio;  // NaN stays
+  const float coef = ratio >= 1.0 ? 1.f : (float)ratio;  // a NaN ratio stays
+  int at = list.n - 1;
   for (uint32_t i = blockIdx.x; i < list.units; i += gridDim.x) {
     const uint32_t unit = list.units - 1 - i;
-    const GradEntry& e = list.e[entry_of(list, unit)];
-    if (coef == 1.f && e.in == e.out && e.in_type == e.out_type) continue;  // in place, nothing to scale
-    const int64_t u = unit - e.unit0;
-    switch (e.in_type * 3 + e.out_type) {
-      case 0: clip_unit<0, 0>(e, u, coef); break;
-      case 1: clip_unit<0, 1>(e, u, coef); break;
-      case 2: clip_unit<0, 2>(e, u, coef); break;
-      case 3: clip_unit<1, 0>(e, u, coef); break;
-      case 4: clip_unit<1, 1>(e, u, coef); break;
-      case 5: clip_unit<1, 2>(e, u, coef); break;
-      case 6: clip_unit<2, 0>(e, u, coef); break;
-      case 7: clip_unit<2, 1>(e, u, coef); break;
-      case 8: clip_unit<2, 2>(e, u, coef); break;
-    }
+    while (list.unit0[at] > unit) --at;
+    const GradEntry& e = list.e[at];
+    if (IN == OUT && coef == 1.f && e.in == e.out) continue;  // in place, nothing to scale
+    clip_unit<IN, OUT>(e, unit - list.unit0[at], coef);
   }
 }
 

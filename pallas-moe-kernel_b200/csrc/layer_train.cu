@@ -27,7 +27,7 @@ static int route_lanes(int E) {
 
 // Blocks per sequence: enough that a warp has one step of tokens, and at most
 // kRouteBlocks over all sequences where a sequence is longer than that.
-constexpr int64_t kRouteBlocks = 148 * 2;
+constexpr int64_t kRouteBlocks = 148 * 4;
 static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
   const int64_t step = kRouteWarps * (32 / route_lanes(E));
   const int64_t most = std::max<int64_t>(1, kRouteBlocks / std::max<int64_t>(1, sequences));
@@ -35,7 +35,7 @@ static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
 }
 
 struct RouteSpace {
-  size_t q, c, z, n, seq, ticket, bytes;
+  size_t q, c, z, n, seq, bytes;
 };
 static RouteSpace route_space(int64_t blocks, int64_t sequences, int E) {
   RouteSpace s;
@@ -47,12 +47,14 @@ static RouteSpace route_space(int64_t blocks, int64_t sequences, int E) {
   };
   s.q = take((size_t)blocks * E * sizeof(float));
   s.c = take((size_t)blocks * E * sizeof(int32_t));
-  s.z = take((size_t)blocks * sizeof(float));
+  s.z = take((size_t)blocks * sizeof(double));
   s.n = take((size_t)blocks * sizeof(int32_t));
-  s.seq = take((size_t)sequences * ((E + 31) / 32) * sizeof(double));
-  s.ticket = take(sizeof(uint32_t));
+  s.seq = take((size_t)sequences * sizeof(double));
   s.bytes = at;
   return s;
+}
+static int64_t route_counters(int64_t chunks, int64_t sequences, int E) {
+  return sequences * route_groups(chunks, E) + sequences + 1;
 }
 
 template <int G, int V, int KMAX>
@@ -68,11 +70,21 @@ static int launch_route_k(const RouteParams& p, int64_t blocks, cudaStream_t st)
   if (p.k <= 8) return launch_route<G, V, 8>(p, blocks, st);
   return launch_route<G, V, 16>(p, blocks, st);
 }
-template <int G, int V>
-static int launch_route_bwd(const RouteBackward& p, int64_t blocks, cudaStream_t st) {
-  route_backward_kernel<G, V><<<(unsigned)blocks, kRouteThreads, 0, st>>>(p);
+template <int G, int V, int KMAX>
+static int launch_backward(const RouteBackward& p, int64_t blocks, cudaStream_t st) {
+  route_backward_kernel<G, V, KMAX><<<(unsigned)blocks, kRouteThreads, 0, st>>>(p);
   MOE_CUDA_TRY(cudaGetLastError());
   return 0;
+}
+template <int G, int V>
+static int launch_backward_k(const RouteBackward& p, int64_t blocks, cudaStream_t st) {
+  if constexpr (G >= kRouteMaxK) {
+    return launch_backward<G, V, kRouteMaxK>(p, blocks, st);  // one slot a lane
+  } else {
+    if (p.k <= 2) return launch_backward<G, V, 2>(p, blocks, st);
+    if (p.k <= 8) return launch_backward<G, V, 8>(p, blocks, st);
+    return launch_backward<G, V, kRouteMaxK>(p, blocks, st);
+  }
 }
 
 static int check_route(int elem_type, int64_t ld, int64_t T, int E, int k, int64_t sequences, int scoring) {
@@ -182,27 +194,33 @@ static int check_tensors(const moe_tensor_desc* t, int n, int norm_type, bool wi
 static int entry_head(const GradEntry& e) {
   const size_t in = reinterpret_cast<uintptr_t>(e.in), out = reinterpret_cast<uintptr_t>(e.out);
   const size_t ib = elem_bytes(e.in_type), ob = elem_bytes(e.out_type);
+  const size_t ce = chunk_elems(e.in_type), store = std::min<size_t>(16, ce * ob);
   if (e.rows > 1)
-    return e.cols % 8 == 0 && in % 16 == 0 && out % 16 == 0 && e.in_ld * ib % 16 == 0 && e.out_ld * ob % 16 == 0 ? 0
-                                                                                                                : -1;
+    return e.cols % ce == 0 && in % 16 == 0 && out % store == 0 && e.in_ld * ib % 16 == 0 && e.out_ld * ob % store == 0
+               ? 0
+               : -1;
   for (int h = 0; h < 8 && h <= e.cols; ++h)
-    if ((in + h * ib) % 16 == 0 && (out + h * ob) % 16 == 0) return h;
+    if ((in + h * ib) % 16 == 0 && (out + h * ob) % store == 0) return h;
   return -1;
 }
 
-// Fills `list` with tensors from *at on; false when none is left.
+// Fills `list` with tensors from *at on (of the pair of types `pair`, or all:
+// -1); false when none is left.
+static int type_pair(const moe_tensor_desc& d) { return d.in_type * 3 + d.out_type; }
 template <int SLOTS>
-static bool fill_list(GradList<SLOTS>& list, const moe_tensor_desc* t, int n, int* at, bool with_out) {
+static bool fill_list(GradList<SLOTS>& list, const moe_tensor_desc* t, int n, int* at, int pair) {
+  const bool with_out = pair >= 0;
   list.n = 0;
   uint64_t units = 0;
   for (; *at < n && list.n < SLOTS; ++*at) {
     const moe_tensor_desc& d = t[*at];
-    if (d.rows == 0 || d.cols == 0) continue;
+    if (d.rows == 0 || d.cols == 0 || (with_out && type_pair(d) != pair)) continue;
     GradEntry& e = list.e[list.n];
     e = GradEntry{d.in, with_out ? d.out : const_cast<void*>(d.in), d.rows, d.cols, d.in_ld,
-                  with_out ? d.out_ld : d.in_ld, d.in_type, with_out ? d.out_type : d.in_type, 0, (uint32_t)units};
-    e.head = entry_head(e);
-    const uint64_t more = ((uint64_t)d.rows * d.cols + kNormUnit - 1) / kNormUnit;
+                  with_out ? d.out_ld : d.in_ld, (int16_t)d.in_type, (int16_t)(with_out ? d.out_type : d.in_type), 0};
+    e.head = (int16_t)entry_head(e);
+    list.unit0[list.n] = (uint32_t)units;
+    const uint64_t per = unit_elems(d.in_type), more = ((uint64_t)d.rows * d.cols + per - 1) / per;
     units += more;
     ++list.n;
   }
@@ -219,7 +237,7 @@ static int launch_partials(const moe_tensor_desc* t, int n, double* partial, int
   int at = 0;
   *count = 0;
   GradList<SLOTS> list;
-  while (fill_list(list, t, n, &at, false)) {
+  while (fill_list(list, t, n, &at, -1)) {
     const int blocks = norm_blocks(list.units, sms);
     norm_partial_kernel<NORM, SLOTS><<<blocks, kNormThreads, 0, st>>>(list, partial + *count);
     MOE_CUDA_TRY(cudaGetLastError());
@@ -227,16 +245,33 @@ static int launch_partials(const moe_tensor_desc* t, int n, double* partial, int
   }
   return 0;
 }
-template <int NORM, int SLOTS>
-static int launch_clip(const moe_tensor_desc* t, int n, ClipNorm c, int sms, cudaStream_t st) {
+template <int SLOTS, int IN, int OUT>
+static int launch_clip_pair(const moe_tensor_desc* t, int n, ClipNorm* c, int sms, cudaStream_t st) {
   int at = 0;
   GradList<SLOTS> list;
-  while (fill_list(list, t, n, &at, true)) {
-    clip_kernel<NORM, SLOTS><<<norm_blocks(list.units, sms), kNormThreads, 0, st>>>(list, c);
+  while (fill_list(list, t, n, &at, IN * 3 + OUT)) {
+    clip_kernel<IN, OUT, SLOTS><<<norm_blocks(list.units, sms), kNormThreads, 0, st>>>(list, *c);
     MOE_CUDA_TRY(cudaGetLastError());
-    c.norm = nullptr;
+    c->norm = nullptr;  // the first launch writes it
   }
   return 0;
+}
+template <int SLOTS>
+static int launch_clip(const moe_tensor_desc* t, int n, ClipNorm c, int sms, cudaStream_t st) {
+  unsigned pairs = 0;
+  for (int i = 0; i < n; ++i)
+    if (t[i].rows && t[i].cols) pairs |= 1u << type_pair(t[i]);
+  int r = 0;
+  if (!r && (pairs & 1u)) r = launch_clip_pair<SLOTS, 0, 0>(t, n, &c, sms, st);
+  if (!r && (pairs & 2u)) r = launch_clip_pair<SLOTS, 0, 1>(t, n, &c, sms, st);
+  if (!r && (pairs & 4u)) r = launch_clip_pair<SLOTS, 0, 2>(t, n, &c, sms, st);
+  if (!r && (pairs & 8u)) r = launch_clip_pair<SLOTS, 1, 0>(t, n, &c, sms, st);
+  if (!r && (pairs & 16u)) r = launch_clip_pair<SLOTS, 1, 1>(t, n, &c, sms, st);
+  if (!r && (pairs & 32u)) r = launch_clip_pair<SLOTS, 1, 2>(t, n, &c, sms, st);
+  if (!r && (pairs & 64u)) r = launch_clip_pair<SLOTS, 2, 0>(t, n, &c, sms, st);
+  if (!r && (pairs & 128u)) r = launch_clip_pair<SLOTS, 2, 1>(t, n, &c, sms, st);
+  if (!r && (pairs & 256u)) r = launch_clip_pair<SLOTS, 2, 2>(t, n, &c, sms, st);
+  return r;
 }
 template <int NORM>
 static int run_norm(const moe_tensor_desc* t, int n, float* norm, double* partial, int sms, cudaStream_t st) {
@@ -244,14 +279,14 @@ static int run_norm(const moe_tensor_desc* t, int n, float* norm, double* partia
   const int r = n <= kGradSlotsSmall ? launch_partials<NORM, kGradSlotsSmall>(t, n, partial, &count, sms, st)
                                      : launch_partials<NORM, kGradSlots>(t, n, partial, &count, sms, st);
   if (r) return r;
-  norm_finish_kernel<NORM><<<1, kNormThreads, 0, st>>>(partial, count, norm);
+  norm_finish_kernel<<<1, kNormThreads, 0, st>>>(NORM, partial, count, norm);
   MOE_CUDA_TRY(cudaGetLastError());
   return 0;
 }
 template <int NORM>
 static int run_clip(const moe_tensor_desc* t, int n, double max_norm, const float* given, float* norm, double* partial,
                     int sms, cudaStream_t st) {
-  ClipNorm c{partial, 0, given, norm, max_norm};
+  ClipNorm c{partial, 0, NORM, given, norm, max_norm};
   const bool small = n <= kGradSlotsSmall;
   if (!given) {
     const int r = small ? launch_partials<NORM, kGradSlotsSmall>(t, n, partial, &c.n, sms, st)
@@ -264,7 +299,7 @@ static int run_clip(const moe_tensor_desc* t, int n, double max_norm, const floa
   } else if (norm && norm != given) {
     MOE_CUDA_TRY(cudaMemcpyAsync(norm, given, sizeof(float), cudaMemcpyDeviceToDevice, st));
   }
-  return small ? launch_clip<NORM, kGradSlotsSmall>(t, n, c, sms, st) : launch_clip<NORM, kGradSlots>(t, n, c, sms, st);
+  return small ? launch_clip<kGradSlotsSmall>(t, n, c, sms, st) : launch_clip<kGradSlots>(t, n, c, sms, st);
 }
 
 }  // namespace moe
@@ -274,6 +309,11 @@ using namespace moe;
 extern "C" {
 
 // ------------------------------------------------------------------ routing
+int64_t moe_route_train_counters(int64_t T, int32_t E, int64_t sequences) {
+  if (T < 0 || E < 1 || E > kRouteMaxExperts || sequences < 1 || T % sequences) return 0;
+  return route_counters(route_chunks(T / sequences, sequences, E), sequences, E);
+}
+
 size_t moe_route_train_workspace_size(int64_t T, int32_t E, int64_t sequences) {
   if (T < 0 || E < 1 || E > kRouteMaxExperts || sequences < 1 || T % sequences) return 0;
   return route_space(route_chunks(T / sequences, sequences, E) * sequences, sequences, E).bytes;
@@ -282,7 +322,7 @@ size_t moe_route_train_workspace_size(int64_t T, int32_t E, int64_t sequences) {
 int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
                     int64_t sequences, const uint8_t* mask, const int32_t* given_ids, int32_t scoring,
                     int32_t normalize, int32_t* ids, float* weights, int32_t* counts, int32_t* tokens, float* balance,
-                    float* z, void* workspace, size_t workspace_bytes, void* stream) {
+                    float* z, void* workspace, size_t workspace_bytes, uint32_t* counters, void* stream) {
   t_err[0] = 0;
   if (int r = check_route(elem_type, ld, T, E, k, sequences, scoring)) return r;
   if (!counts || !tokens || !balance || !z) return fail(MOE_ERR_INVALID_ARG, "null pointer");
@@ -294,7 +334,7 @@ int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T
     MOE_CUDA_TRY(cudaMemsetAsync(z, 0, sizeof(float), st));
     return 0;
   }
-  if (!logits || !ids || !weights) return fail(MOE_ERR_INVALID_ARG, "null pointer");
+  if (!logits || !ids || !weights || !counters) return fail(MOE_ERR_INVALID_ARG, "null pointer");
   if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(elem_type))
     return fail(MOE_ERR_MISALIGNED, "logits are not aligned to their elements");
   const int64_t seq_len = T / sequences, chunks = route_chunks(seq_len, sequences, E), blocks = chunks * sequences;
@@ -315,9 +355,15 @@ int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T
   p.weights = weights;
   p.part_q = reinterpret_cast<float*>(w + s.q);
   p.part_c = reinterpret_cast<int32_t*>(w + s.c);
-  p.part_z = reinterpret_cast<float*>(w + s.z);
+  p.part_z = reinterpret_cast<double*>(w + s.z);
   p.part_n = reinterpret_cast<int32_t*>(w + s.n);
-  p.ticket = reinterpret_cast<uint32_t*>(w + s.ticket);
+  p.seq_part = reinterpret_cast<double*>(w + s.seq);
+  p.counts = counts;
+  p.tokens = tokens;
+  p.balance = balance;
+  p.z = z;
+  p.counters = counters;
+  p.S = (int32_t)sequences;
   p.ld = ld;
   p.seq_len = seq_len;
   p.chunks = (int32_t)chunks;
@@ -327,39 +373,16 @@ int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T
   p.vec = route_vec(logits, ld, E, elem_type);
   p.sigmoid = scoring == MOE_SCORE_SIGMOID;
   p.normalize = normalize != 0;
-  int r = 0;
-  if (E > 512) r = launch_route_k<32, 32>(p, blocks, st);
-  else if (E > 256) r = launch_route_k<32, 16>(p, blocks, st);
-  else switch (route_lanes(E)) {
-    case 1: r = launch_route_k<1, 8>(p, blocks, st); break;
-    case 2: r = launch_route_k<2, 8>(p, blocks, st); break;
-    case 4: r = launch_route_k<4, 8>(p, blocks, st); break;
-    case 8: r = launch_route_k<8, 8>(p, blocks, st); break;
-    case 16: r = launch_route_k<16, 8>(p, blocks, st); break;
-    default: r = launch_route_k<32, 8>(p, blocks, st); break;
+  if (E > 512) return launch_route_k<32, 32>(p, blocks, st);
+  if (E > 256) return launch_route_k<32, 16>(p, blocks, st);
+  switch (route_lanes(E)) {
+    case 1: return launch_route_k<1, 8>(p, blocks, st);
+    case 2: return launch_route_k<2, 8>(p, blocks, st);
+    case 4: return launch_route_k<4, 8>(p, blocks, st);
+    case 8: return launch_route_k<8, 8>(p, blocks, st);
+    case 16: return launch_route_k<16, 8>(p, blocks, st);
   }
-  if (r) return r;
-  RouteFinish f{};
-  f.part_q = p.part_q;
-  f.part_c = p.part_c;
-  f.part_z = p.part_z;
-  f.part_n = p.part_n;
-  f.ticket = p.ticket;
-  f.seq_part = reinterpret_cast<double*>(w + s.seq);
-  f.counts = counts;
-  f.tokens = tokens;
-  f.balance = balance;
-  f.z = z;
-  f.S = (int32_t)sequences;
-  f.chunks = (int32_t)chunks;
-  f.E = E;
-  f.k = k;
-  f.eblocks = (E + 31) / 32;
-  if (sequences * f.eblocks > (int64_t)0x7fffffff)
-    return fail(MOE_ERR_UNSUPPORTED_SHAPE, "%lld sequences of E=%d", (long long)sequences, E);
-  route_finish_kernel<<<(unsigned)(sequences * f.eblocks), kFinishThreads, 0, st>>>(f);
-  MOE_CUDA_TRY(cudaGetLastError());
-  return 0;
+  return launch_route_k<32, 8>(p, blocks, st);
 }
 
 int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
@@ -399,16 +422,16 @@ int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_
   p.sigmoid = scoring == MOE_SCORE_SIGMOID;
   p.normalize = normalize != 0;
   const int64_t blocks = p.chunks * sequences;
-  if (E > 512) return launch_route_bwd<32, 32>(p, blocks, st);
-  if (E > 256) return launch_route_bwd<32, 16>(p, blocks, st);
+  if (E > 512) return launch_backward_k<32, 32>(p, blocks, st);
+  if (E > 256) return launch_backward_k<32, 16>(p, blocks, st);
   switch (route_lanes(E)) {
-    case 1: return launch_route_bwd<1, 8>(p, blocks, st);
-    case 2: return launch_route_bwd<2, 8>(p, blocks, st);
-    case 4: return launch_route_bwd<4, 8>(p, blocks, st);
-    case 8: return launch_route_bwd<8, 8>(p, blocks, st);
-    case 16: return launch_route_bwd<16, 8>(p, blocks, st);
+    case 1: return launch_backward_k<1, 8>(p, blocks, st);
+    case 2: return launch_backward_k<2, 8>(p, blocks, st);
+    case 4: return launch_backward_k<4, 8>(p, blocks, st);
+    case 8: return launch_backward_k<8, 8>(p, blocks, st);
+    case 16: return launch_backward_k<16, 8>(p, blocks, st);
   }
-  return launch_route_bwd<32, 8>(p, blocks, st);
+  return launch_backward_k<32, 8>(p, blocks, st);
 }
 
 // ------------------------------------------------------------------ rows

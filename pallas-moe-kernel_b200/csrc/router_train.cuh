@@ -23,9 +23,17 @@
 // Layout: G lanes hold one row, V consecutive experts each (G V >= E), so
 // small E packs 32 / G tokens in a warp and the expert order is the lane
 // order: among equal maxima the lowest lane, then the lowest element, is the
-// lowest id.  Sums over tokens stay in registers, then go warp by warp and
-// block by block in a fixed order: no float atomics, results repeat bit for
-// bit.  A block's tokens belong to one sequence.
+// lowest id.  Slot j of a row (its j-th choice) lives in lane j % G, so that
+// ids, weights and their gradients move coalesced and their exponentials run
+// side by side.  Exponentials are 2^(x log2 e) with the row maximum taken off
+// before the rounding.
+//
+// Sums over tokens stay in registers, then go warp by warp and block by block
+// in a fixed order: no float atomics, results repeat bit for bit.  A block's
+// tokens belong to one sequence.  The blocks that finish last add up what the
+// others wrote - 16 blocks, then a sequence, then all - found by counters that
+// are zero between calls, which saves a second launch (9 us of a 15 us
+// forward at T = 16384, E = 8).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,6 +49,7 @@ enum : int { kElemF32 = 0, kElemBF16 = 1, kElemF16 = 2 };
 
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteGroup = 16;  // blocks whose sums are added first
 
 struct RouteParams {
   const void* logits;      // (T, E), rows `ld` elements apart
@@ -48,14 +57,19 @@ struct RouteParams {
   const int32_t* given;    // (T, k) or null: ids chosen by the caller
   int32_t* ids;            // (T, k)
   float* weights;          // (T, k)
+  int32_t* counts;         // (S, E)
+  int32_t* tokens;         // (S,)
+  float* balance;
+  float* z;
   float* part_q;           // [blocks][E] sums of q
   int32_t* part_c;         // [blocks][E] counts
-  float* part_z;           // [blocks] sums of lse^2
+  double* part_z;          // [blocks] sums of lse^2
   int32_t* part_n;         // [blocks] tokens
-  uint32_t* ticket;        // zeroed here for route_finish_kernel
+  double* seq_part;        // [S] sum of c_e P_e terms
+  uint32_t* counters;      // [S groups][S][1], zero before and after
   int64_t ld;
   int64_t seq_len;         // tokens per sequence
-  int32_t chunks;          // blocks per sequence
+  int32_t S, chunks;       // sequences, blocks per sequence
   int32_t E, k;
   int32_t type;            // kElem* of the logits
   int32_t vec;             // rows can be read in 16-byte vectors (8 elements at a time)
@@ -114,27 +128,61 @@ __device__ __forceinline__ void elem_store(void* p, int type, int64_t i, float v
   else static_cast<uint16_t*>(p)[i] = elem_bits16(v, type);
 }
 
-// Experts [e0, e0 + V) of the row at element offset `row`; -inf past E.
-template <int V>
-__device__ __forceinline__ void row_load(const void* p, int type, int vec, int64_t row, int e0, int E, bool live,
-                                         float (&v)[V]) {
+// Experts [e0, e0 + V) of the row at element offset `row`; -inf past E.  The
+// types are told apart once per row: a choice inside the conversions costs
+// more than they do.
+template <int TYPE, int V>
+__device__ __forceinline__ void row_load_t(const void* p, int vec, int64_t row, int e0, int E, bool live,
+                                           float (&v)[V]) {
 #pragma unroll
   for (int c = 0; c < V; c += 8) {
     if (live && vec && e0 + c < E) {
-      elem_load8(p, type, row + e0 + c, v + c);
+      elem_load8(p, TYPE, row + e0 + c, v + c);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        v[c + i] = live && e0 + c + i < E ? elem_load(p, type, row + e0 + c + i) : -INFINITY;
+        v[c + i] = live && e0 + c + i < E ? elem_load(p, TYPE, row + e0 + c + i) : -INFINITY;
     }
   }
+}
+template <int V>
+__device__ __forceinline__ void row_load(const void* p, int type, int vec, int64_t row, int e0, int E, bool live,
+                                         float (&v)[V]) {
+  if (type == kElemF32) row_load_t<kElemF32>(p, vec, row, e0, E, live, v);
+  else if (type == kElemBF16) row_load_t<kElemBF16>(p, vec, row, e0, E, live, v);
+  else row_load_t<kElemF16>(p, vec, row, e0, E, live, v);
+}
+template <int TYPE, int V>
+__device__ __forceinline__ void row_put_t(void* p, int vec, int64_t row, int e0, int E, const float (&v)[V]) {
+#pragma unroll
+  for (int c = 0; c < V; c += 8) {
+    if (vec) {
+      if (e0 + c < E) elem_store8(p, TYPE, row + e0 + c, v + c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (e0 + c + i < E) elem_store(p, TYPE, row + e0 + c + i, v[c + i]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void row_put(void* p, int type, int vec, int64_t row, int e0, int E, const float (&v)[V]) {
+  if (type == kElemF32) row_put_t<kElemF32>(p, vec, row, e0, E, v);
+  else if (type == kElemBF16) row_put_t<kElemBF16>(p, vec, row, e0, E, v);
+  else row_put_t<kElemF16>(p, vec, row, e0, E, v);
 }
 
 template <int G>
 __device__ __forceinline__ float group_max(float v) {
+  if constexpr (G == 32) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+  } else {
 #pragma unroll
-  for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+    for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
 }
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -143,36 +191,297 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// s_e e^-m with m = min(row maximum, 0): sigmoid scores of a row scaled so
-// that a row of very negative logits keeps its ratios (unscaled, all of them
-// would leave the f32 range).  r = e^(m - l) is kept for the slope.
-struct SigmoidRow {
-  float m, em;
-  __device__ __forceinline__ explicit SigmoidRow(float mx) : m(fminf(mx, 0.f)), em(expf(fminf(mx, 0.f))) {}
-  __device__ __forceinline__ float r(float l) const { return expf(m - l); }
-  __device__ __forceinline__ float scaled(float r_) const { return 1.f / (em + r_); }
-  // 1 - s = r / (e^m + r); r is infinite far below the maximum, where it is 1.
-  __device__ __forceinline__ float slope(float r_) const { return r_ > 1e37f ? 1.f : r_ / (em + r_); }
-};
+// ---------------------------------------------------------------- scores
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// Flushing forms: a result below 2^-126 is 0, which spares the rescaling that
+// the others spend three instructions on.
+__device__ __forceinline__ float lg2_ftz(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int V>
+__device__ __forceinline__ float lane_max(const float (&v)[V]) {
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < V; ++i) m = fmaxf(m, v[i]);
+  return m;
+}
+
+// e_i = 2^(l_i log2 e - mxl), mxl = the row maximum times log2 e, rounded: one
+// factor near 1 in all of them, which the ratios p = e / sum(e) and
+// lse = (mxl + log2 sum(e)) ln 2 are free of.  Rows that are not kept have
+// l = -inf throughout, and e = 0.
+template <int V>
+__device__ __forceinline__ float row_exp(const float (&v)[V], float mxl, float (&e)[V]) {
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    e[i] = ex2_ftz(fmaf(v[i], kLog2e, -mxl));
+    total += e[i];
+  }
+  return total;
+}
+
+// Sigmoid scores from the same exponentials.  For a maximum mx >= 0,
+// s = e / (e + 2^-mxl); for mx < 0 every s is small and is kept as
+// s' = s 2^-mxl = e / (e 2^mxl + 1), so that a row of very negative logits has
+// ratios at all.  Both are s' = e t with t = 1 / (e a + b), and 1 - s = b t.
+// Above mx = 40, e would lose scores near 0 logits: they get exponentials of
+// their own.  `ds` receives s' (1 - s), the derivative.
+template <int V>
+__device__ __forceinline__ void row_sigmoid(const float (&v)[V], const float (&e)[V], float mx, float mxl,
+                                            float (&s)[V], float (&ds)[V]) {
+  if (mx > 40.f) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float r = ex2_ftz(-kLog2e * v[i]);
+      s[i] = rcp_ftz(1.f + r);
+      ds[i] = r > 1e18f ? s[i] : r * s[i] * s[i];
+    }
+    return;
+  }
+  const float a = mx >= 0.f ? 1.f : ex2_ftz(mxl), b = mx >= 0.f ? ex2_ftz(-mxl) : 1.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float t = rcp_ftz(fmaf(e[i], a, b));
+    s[i] = e[i] * t;
+    ds[i] = s[i] * (b * t);
+  }
+}
+
+// The score of a chosen logit relative to `top`: e^(l - top), or a sigmoid
+// times e^-min(top, 0).
+__device__ __forceinline__ float slot_score(float l, float top, bool sigmoid) {
+  if (!sigmoid) return ex2_ftz((l - top) * kLog2e);
+  const float m = fminf(top, 0.f);
+  return rcp_ftz(ex2_ftz(m * kLog2e) + ex2_ftz((m - l) * kLog2e));
+}
 
 // ---------------------------------------------------------------- forward
-// Bounded by instruction issue rather than HBM at E = 256, k = 8 (k rounds of
-// a maximum over the row); see the launch code for the group sizes.
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Sum over the block, valid in every thread; s_w holds one value per warp.
+__device__ __forceinline__ double block_sum(double v, double* s_w) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  v = warp_sum(v);
+  __syncthreads();
+  if (lane == 0) s_w[warp] = v;
+  __syncthreads();
+  double sum = 0.0;
+  for (int w = 0; w < nw; ++w) sum += s_w[w];
+  return sum;
+}
+
+
+// Three of them at once; s_w holds three values per warp.
+__device__ __forceinline__ void block_sum3(double& a, double& b, double& c, double* s_w) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  a = warp_sum(a);
+  b = warp_sum(b);
+  c = warp_sum(c);
+  __syncthreads();
+  if (lane == 0) {
+    s_w[warp] = a;
+    s_w[nw + warp] = b;
+    s_w[2 * nw + warp] = c;
+  }
+  __syncthreads();
+  a = b = c = 0.0;
+  for (int w = 0; w < nw; ++w) {
+    a += s_w[w];
+    b += s_w[nw + w];
+    c += s_w[2 * nw + w];
+  }
+}
+
+// Whether this block is the last of `n` to come to `counter`, which it then
+// sets back to 0.  Called by the whole block after its global writes.
+__device__ __forceinline__ bool last_block(uint32_t* counter, uint32_t n, int* s_flag) {
+  if (n == 1) {
+    __syncthreads();
+    return true;
+  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = atomicAdd(counter, 1u) == n - 1;
+    if (last) *counter = 0;
+    *s_flag = last;
+  }
+  __syncthreads();
+  __threadfence();
+  return *s_flag != 0;
+}
+
+// Groups of blocks whose sums are added first: where a sequence has so many
+// blocks and experts that its last block alone would read more than 8 rows a
+// thread, which it has in flight together.
+__host__ __device__ __forceinline__ int route_groups(int64_t chunks, int E) {
+  return chunks * E > 8 * kRouteThreads ? (int)((chunks + kRouteGroup - 1) / kRouteGroup) : 1;
+}
+
+// Adds up blocks' sums, as far as this block is the last one to finish.
+__device__ __forceinline__ void route_finish(const RouteParams& p, int64_t seq, int chunk, double* s_w, double* s_q, int* s_c,
+                                             int* s_flag) {
+  const int E = p.E, tid = threadIdx.x;
+  const int groups = route_groups(p.chunks, E);
+  const int64_t b0 = seq * p.chunks;
+  uint32_t* seq_counters = p.counters + (int64_t)p.S * groups;
+  int stride = 1, rows = p.chunks;
+  if (groups > 1) {
+    const int g = chunk / kRouteGroup;
+    const int64_t r0 = b0 + (int64_t)g * kRouteGroup;
+    const int n = min(kRouteGroup, p.chunks - g * kRouteGroup);
+    if (!last_block(p.counters + seq * groups + g, n, s_flag)) return;
+    for (int e = tid; e < E; e += kRouteThreads) {
+      float q[kRouteGroup];
+      int c[kRouteGroup];
+#pragma unroll
+      for (int i = 0; i < kRouteGroup; ++i) {
+        q[i] = i < n ? __ldcg(p.part_q + (r0 + i) * E + e) : 0.f;
+        c[i] = i < n ? __ldcg(p.part_c + (r0 + i) * E + e) : 0;
+      }
+#pragma unroll
+      for (int i = 1; i < kRouteGroup; ++i) {
+        q[0] += q[i];
+        c[0] += c[i];
+      }
+      p.part_q[r0 * E + e] = q[0];
+      p.part_c[r0 * E + e] = c[0];
+    }
+    if (tid < 32) {
+      double z = tid < n ? __ldcg(p.part_z + r0 + tid) : 0.0;
+      int m = tid < n ? __ldcg(p.part_n + r0 + tid) : 0;
+#pragma unroll
+      for (int o = 8; o; o >>= 1) {
+        z += __shfl_xor_sync(0xffffffffu, z, o);
+        m += __shfl_xor_sync(0xffffffffu, m, o);
+      }
+      if (tid == 0) {
+        p.part_z[r0] = z;
+        p.part_n[r0] = m;
+      }
+    }
+    stride = kRouteGroup;
+    rows = groups;
+  }
+  if (!last_block(seq_counters + seq, rows, s_flag)) return;
+  double z = 0.0, n = 0.0, sum = 0.0;
+  for (int i = tid; i < rows; i += kRouteThreads) {
+    z += __ldcg(p.part_z + b0 + (int64_t)i * stride);
+    n += __ldcg(p.part_n + b0 + (int64_t)i * stride);
+  }
+  // `parts` threads take an expert's rows in turn (few experts: many threads
+  // each), neighbouring threads neighbouring experts.
+  int width = 1;
+  while (width < E && width < kRouteThreads) width *= 2;
+  const int parts = kRouteThreads / width, part = tid / width;
+  for (int e = tid % width; e < E; e += width) {
+    double q = 0.0;
+    int c = 0;
+    for (int i0 = part; i0 < rows; i0 += 8 * parts) {
+      float qs[8];
+      int cs[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * parts;
+        qs[u] = i < rows ? __ldcg(p.part_q + (b0 + (int64_t)i * stride) * E + e) : 0.f;
+        cs[u] = i < rows ? __ldcg(p.part_c + (b0 + (int64_t)i * stride) * E + e) : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        q += (double)qs[u];
+        c += cs[u];
+      }
+    }
+    if (parts > 1) {  // then E <= width: every thread comes by at most once
+      s_q[tid] = q;
+      s_c[tid] = c;
+    } else {
+      p.counts[seq * E + e] = c;
+      sum += (double)c * q;
+    }
+  }
+  if (parts > 1) {
+    __syncthreads();
+    if (tid < E) {
+      double q = 0.0;
+      int c = 0;
+      for (int i = 0; i < parts; ++i) {
+        q += s_q[i * width + tid];
+        c += s_c[i * width + tid];
+      }
+      p.counts[seq * E + tid] = c;
+      sum = (double)c * q;
+    }
+  }
+  block_sum3(sum, z, n, s_w);
+  if (tid == 0) {
+    p.tokens[seq] = (int)n;
+    sum = n > 0.0 ? sum * E / (p.k * n * n) : 0.0;
+    if (p.S == 1) {
+      *p.balance = (float)sum;
+      *p.z = (float)(n > 0.0 ? z / n : 0.0);
+    } else {
+      p.seq_part[seq] = sum;
+      p.part_z[b0] = z;
+    }
+  }
+  if (p.S == 1 || !last_block(seq_counters + p.S, p.S, s_flag)) return;
+  double bal = 0.0, live = 0.0;
+  z = n = 0.0;
+  for (int64_t i = tid; i < p.S; i += kRouteThreads) {
+    const int ns = __ldcg(p.tokens + i);
+    bal += __ldcg(p.seq_part + i);
+    z += __ldcg(p.part_z + i * p.chunks);
+    n += ns;
+    live += ns > 0;
+  }
+  live = block_sum(live, s_w);
+  block_sum3(bal, z, n, s_w);
+  if (tid == 0) {
+    *p.balance = (float)(live > 0.0 ? bal / live : 0.0);
+    *p.z = (float)(n > 0.0 ? z / n : 0.0);
+  }
+}
+
 template <int G, int V, int KMAX>
 __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteParams p) {
-  constexpr int TPW = 32 / G;  // tokens per warp and step
-  extern __shared__ int s_cnt[];  // [E] counts, then [warps][G V] sums of q
-  __shared__ float s_z[kRouteWarps];
+  constexpr int TPW = 32 / G;                // tokens per warp and step
+  constexpr int KS = (KMAX + G - 1) / G;     // slots per lane
+  extern __shared__ int s_cnt[];             // [E] counts, then [warps][G V] sums of q
+  __shared__ double s_w[3 * kRouteWarps];
+  __shared__ double s_fq[kRouteThreads];
+  __shared__ int s_fc[kRouteThreads];
+  __shared__ double s_z[kRouteWarps];
   __shared__ int s_n[kRouteWarps];
+  __shared__ int s_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gl = lane % G;
-  const uint32_t gmask = (G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (lane / G * G));
+  const uint32_t gmask = (G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << (lane / G * G));
   const int e0 = gl * V, E = p.E, k = p.k;
   for (int e = threadIdx.x; e < E; e += kRouteThreads) s_cnt[e] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
   __syncthreads();
 
-  const int64_t seq = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
+  const int64_t seq = blockIdx.x / p.chunks;
+  const int chunk = blockIdx.x % p.chunks;
   const int64_t lo = seq * p.seq_len + p.seq_len * chunk / p.chunks;
   const int64_t hi = seq * p.seq_len + p.seq_len * (chunk + 1) / p.chunks;
   float acc[V];
@@ -186,105 +495,111 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
     const bool live = inside && (!p.mask || __ldg(p.mask + t));
     float v[V];
     row_load<V>(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
-    float mx = v[0];
+    int id[KS];
+    float sel[KS];
+    if (p.given) {
 #pragma unroll
-    for (int i = 1; i < V; ++i) mx = fmaxf(mx, v[i]);
-    mx = group_max<G>(mx);
-    const bool keep = mx > -INFINITY;
-    float ex[V], total = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      ex[i] = keep && e0 + i < E ? expf(v[i] - mx) : 0.f;
-      total += ex[i];
-    }
-    total = group_sum<G>(total);
-    const float lse = keep ? mx + logf(total) : 0.f;
-    const SigmoidRow sg(mx);
-    float norm = total;  // what the scores are divided by to give q
-    if (p.sigmoid) {
-      norm = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        ex[i] = keep && e0 + i < E ? sg.scaled(sg.r(v[i])) : 0.f;
-        norm += ex[i];
+      for (int s = 0; s < KS; ++s) {
+        const int j = s * G + gl;
+        id[s] = live && j < k ? __ldg(p.given + t * k + j) : -1;
+        if (id[s] < 0 || id[s] >= E) id[s] = -1;
+        sel[s] = id[s] >= 0 ? elem_load(p.logits, p.type, t * p.ld + id[s]) : -INFINITY;
       }
-      norm = group_sum<G>(norm);
     }
-    const float inv = keep ? 1.f / norm : 0.f;
+    float m = lane_max(v);
+    const float mx = group_max<G>(m);
+    const bool keep = mx > -INFINITY;
+    if (!keep) {  // a row of NaN takes no part either
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] += ex[i] * inv;
-    if (gl == 0 && keep) {
-      z += lse * lse;
-      ++n;
+      for (int i = 0; i < V; ++i) v[i] = -INFINITY;
+    }
+    const float mxl = keep ? mx * kLog2e : 0.f;
+    float ex[V];
+    const float total = group_sum<G>(row_exp(v, mxl, ex));
+    const float lse = keep ? (mxl + lg2_ftz(total)) * kLn2 : 0.f;
+    z += lse * lse;
+    n += keep;
+    float inv;  // 1 / the sum of the scores
+    if (!p.sigmoid) {
+      inv = keep ? 1.f / total : 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(ex[i], inv, acc[i]);
+    } else {
+      float sc[V], ds[V], sum = 0.f;
+      row_sigmoid(v, ex, mx, mxl, sc, ds);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += sc[i];
+      sum = group_sum<G>(sum);
+      inv = keep ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(sc[i], inv, acc[i]);
     }
 
-    // Choice: k rounds of the row's maximum, or the caller's ids.
-    float sel[KMAX];
+    // Choice: k rounds of the row's maximum.
     if (!p.given) {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = v[i] > -INFINITY ? v[i] : -INFINITY;  // NaN is never chosen
+      m = lane_max(v);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        id[s] = -1;
+        sel[s] = -INFINITY;
+      }
 #pragma unroll
       for (int j = 0; j < KMAX; ++j) {
         if (j >= k) break;
-        float m = v[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) m = fmaxf(m, v[i]);
         const float M = group_max<G>(m);
-        const bool any = M > -INFINITY;
-        const uint32_t owners = __ballot_sync(0xffffffffu, m == M) & gmask;
-        int id = -1;
-        if (lane == __ffs(owners) - 1) {
-          if (any) {
+        const uint32_t owners = __ballot_sync(0xffffffffu, m == M && M > -INFINITY) & gmask;
+        const int owner = __ffs(owners) - 1;
+        int at = -1;
+        if (lane == owner) {
 #pragma unroll
-            for (int i = V - 1; i >= 0; --i)
-              if (v[i] == M) id = i;
+          for (int i = V - 1; i >= 0; --i)
+            if (v[i] == M) at = i;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (i == id) v[i] = -INFINITY;
-            id += e0;
-            atomicAdd(&s_cnt[id], 1);
-          }
-          if (inside) p.ids[t * k + j] = id;
+          for (int i = 0; i < V; ++i)
+            if (i == at) v[i] = -INFINITY;
+          m = lane_max(v);
+          at += e0;
         }
-        sel[j] = M;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < KMAX; ++j) {
-        if (j >= k) break;
-        int id = live ? __ldg(p.given + t * k + j) : -1;
-        if (!keep || id < 0 || id >= E) id = -1;
-        sel[j] = id >= 0 ? elem_load(p.logits, p.type, t * p.ld + id) : -INFINITY;
-        if (gl == 0 && inside) {
-          p.ids[t * k + j] = id;
-          if (id >= 0) atomicAdd(&s_cnt[id], 1);
+        at = __shfl_sync(0xffffffffu, at, owner < 0 ? lane : owner);
+        if (gl == j % G) {
+          id[j / G] = at;
+          sel[j / G] = M;
         }
       }
     }
-    // Weights of the chosen logits, on the row's own scale; normalised, the
-    // softmax is taken relative to the largest chosen logit.
-    float top = mx, sum = 0.f;
+    // Weights of the chosen logits, on the row's own scale; those that the
+    // caller chose, normalised, relative to the largest of them.
+    float top = mx;
+    if (p.given && p.normalize) {
+      top = sel[0];
+#pragma unroll
+      for (int s = 1; s < KS; ++s) top = fmaxf(top, sel[s]);
+      top = group_max<G>(top);
+    }
+    float w[KS], sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      // -inf: no expert in this slot, or one chosen by the caller with score 0.
+      w[s] = keep && sel[s] > -INFINITY ? slot_score(sel[s], top, p.sigmoid) : 0.f;
+      if (sel[s] != sel[s]) w[s] = sel[s];
+      sum += w[s];
+    }
+    float scale = p.sigmoid ? ex2_ftz(fminf(mx, 0.f) * kLog2e) : inv;
     if (p.normalize) {
-      top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < KMAX; ++j)
-        if (j < k) top = fmaxf(top, sel[j]);
+      sum = group_sum<G>(sum);
+      scale = sum == 0.f ? 0.f : 1.f / sum;
     }
-    const SigmoidRow sw(top);
 #pragma unroll
-    for (int j = 0; j < KMAX; ++j) {
-      if (j >= k) break;
-      // A chosen -inf (the caller's choice) has score 0; a slot without an
-      // expert has sel = -inf as well.
-      if (sel[j] == -INFINITY) sel[j] = 0.f;
-      else sel[j] = p.sigmoid ? sw.scaled(sw.r(sel[j])) : expf(sel[j] - top);
-      sum += sel[j];
-    }
-    const float scale = p.normalize ? (sum == 0.f ? 0.f : 1.f / sum) : p.sigmoid ? sw.em : inv;
-#pragma unroll
-    for (int j = 0; j < KMAX; ++j) {
-      if (j >= k) break;
-      if (gl == j % G && inside) p.weights[t * k + j] = sel[j] * scale;
+    for (int s = 0; s < KS; ++s) {
+      const int j = s * G + gl;
+      if (inside && j < k) {
+        if (!keep) id[s] = -1;
+        p.ids[t * k + j] = id[s];
+        p.weights[t * k + j] = keep ? w[s] * scale : 0.f;
+        if (id[s] >= 0) atomicAdd(&s_cnt[id[s]], 1);
+      }
     }
   }
 
@@ -293,9 +608,6 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
   for (int o = G; o < 32; o <<= 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
     z += __shfl_xor_sync(0xffffffffu, z, o);
     n += __shfl_xor_sync(0xffffffffu, n, o);
   }
@@ -317,7 +629,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
     p.part_c[(int64_t)blockIdx.x * E + e] = s_cnt[e];
   }
   if (threadIdx.x == 0) {
-    float zs = 0.f;
+    double zs = 0.0;
     int ns = 0;
     for (int w = 0; w < kRouteWarps; ++w) {
       zs += s_z[w];
@@ -326,102 +638,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
     p.part_z[blockIdx.x] = zs;
     p.part_n[blockIdx.x] = ns;
   }
-}
-
-// ---------------------------------------------------------------- finish
-// Block (s, b): experts [32 b, 32 b + 32) of sequence s: counts, and the
-// block's part of sum_e c_e P_e.  The block that finishes last adds the parts
-// of all sequences in order (f64: the sums run over every block).
-struct RouteFinish {
-  const float* part_q;
-  const int32_t* part_c;
-  const float* part_z;
-  const int32_t* part_n;
-  uint32_t* ticket;
-  double* seq_part;   // [S][blocks per sequence]
-  int32_t* counts;    // (S, E)
-  int32_t* tokens;    // (S,)
-  float* balance;
-  float* z;
-  int32_t S, chunks, E, k, eblocks;
-};
-
-constexpr int kFinishThreads = 512;
-
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-// Sum over the block, valid in every thread; s_w holds one value per warp.
-__device__ __forceinline__ double block_sum(double v, double* s_w) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  v = warp_sum(v);
-  __syncthreads();
-  if (lane == 0) s_w[warp] = v;
-  __syncthreads();
-  double sum = 0.0;
-  for (int w = 0; w < nw; ++w) sum += s_w[w];
-  return sum;
-}
-
-__global__ void __launch_bounds__(kFinishThreads) route_finish_kernel(const RouteFinish p) {
-  constexpr int R = kFinishThreads / 32;  // partial rows read at a time
-  __shared__ double s_q[R][32];
-  __shared__ int s_c[R][32];
-  __shared__ double s_w[R];
-  __shared__ int s_last;
-  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int s = blockIdx.x / p.eblocks, eb = blockIdx.x % p.eblocks;
-  const int e = eb * 32 + lane;
-  const int64_t b0 = (int64_t)s * p.chunks;
-  double q = 0.0;
-  int c = 0;
-  if (e < p.E) {
-    for (int i = r; i < p.chunks; i += R) {
-      q += (double)p.part_q[(b0 + i) * p.E + e];
-      c += p.part_c[(b0 + i) * p.E + e];
-    }
-  }
-  double n = 0.0;
-  for (int i = threadIdx.x; i < p.chunks; i += kFinishThreads) n += p.part_n[b0 + i];
-  n = block_sum(n, s_w);
-  s_q[r][lane] = q;
-  s_c[r][lane] = c;
-  __syncthreads();
-  if (r == 0) {
-    for (int i = 1; i < R; ++i) {
-      q += s_q[i][lane];
-      c += s_c[i][lane];
-    }
-    if (e < p.E) p.counts[(int64_t)s * p.E + e] = c;
-    const double sum = warp_sum(n > 0.0 ? (double)c * p.E / (p.k * n) * (q / n) : 0.0);
-    if (lane == 0) {
-      p.seq_part[blockIdx.x] = sum;
-      if (eb == 0) p.tokens[s] = (int)n;
-      __threadfence();
-      s_last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
-    }
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  double bal = 0.0, z = 0.0, tokens = 0.0, live = 0.0;
-  for (int64_t i = threadIdx.x; i < (int64_t)p.S * p.eblocks; i += kFinishThreads) bal += __ldcg(p.seq_part + i);
-  for (int64_t i = threadIdx.x; i < (int64_t)p.S * p.chunks; i += kFinishThreads) z += p.part_z[i];
-  for (int i = threadIdx.x; i < p.S; i += kFinishThreads) {
-    const int ns = __ldcg(p.tokens + i);
-    tokens += ns;
-    live += ns > 0;
-  }
-  bal = block_sum(bal, s_w);
-  z = block_sum(z, s_w);
-  tokens = block_sum(tokens, s_w);
-  live = block_sum(live, s_w);
-  if (threadIdx.x == 0) {
-    *p.balance = (float)(live > 0.0 ? bal / live : 0.0);
-    *p.z = (float)(tokens > 0.0 ? z / tokens : 0.0);
-  }
+  route_finish(p, seq, chunk, s_w, s_fq, s_fc, &s_flag);
 }
 
 // ---------------------------------------------------------------- backward
@@ -445,48 +662,47 @@ struct RouteBackward {
 //   normalised                   w_j (dw_j - <dw, w>) (times 1 - s_j, sigmoid)
 //   plain softmax probability    w_j dw_j, and -p_e <dw, w> on every expert
 //   plain sigmoid                w_j dw_j (1 - s_j)
-template <int G, int V>
+// It is formed in the slots' lanes and handed to the experts' lanes through a
+// row in shared memory that is zero between uses (a register exchange takes
+// k V compares a lane).
+template <int G, int V, int KMAX>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteBackward p) {
   constexpr int TPW = 32 / G;
-  __shared__ int s_sum[2][kRouteWarps];
+  constexpr int KS = (KMAX + G - 1) / G;
+  __shared__ __align__(16) float s_row[kRouteWarps][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gl = lane % G;
   const int e0 = gl * V, E = p.E, k = p.k;
-  const int64_t seq = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
+  const int64_t seq = blockIdx.x / p.chunks;
+  const int chunk = blockIdx.x % p.chunks;
   const int64_t lo = seq * p.seq_len + p.seq_len * chunk / p.chunks;
   const int64_t hi = seq * p.seq_len + p.seq_len * (chunk + 1) / p.chunks;
+  float* row = s_row[warp] + (lane / G) * (G * V);
+#pragma unroll
+  for (int i = 0; i < V; ++i) s_row[warp][i * 32 + lane] = 0.f;
+  __syncwarp();
 
   // Tokens in all sequences and sequences with any.
-  int all = 0, live_seqs = 0;
-  for (int i = threadIdx.x; i < p.S; i += kRouteThreads) {
-    const int ns = __ldg(p.tokens + i);
-    all += ns;
-    live_seqs += ns > 0;
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    live_seqs += __shfl_xor_sync(0xffffffffu, live_seqs, o);
-  }
-  if (lane == 0) {
-    s_sum[0][warp] = all;
-    s_sum[1][warp] = live_seqs;
-  }
-  __syncthreads();
-  all = live_seqs = 0;
-  for (int w = 0; w < kRouteWarps; ++w) {
-    all += s_sum[0][w];
-    live_seqs += s_sum[1][w];
-  }
   const int ns = __ldg(p.tokens + seq);
+  int all = ns, live_seqs = ns > 0;
+  if (p.S > 1) {
+    all = live_seqs = 0;
+    for (int i = lane; i < p.S; i += 32) {
+      const int m = __ldg(p.tokens + i);
+      all += m;
+      live_seqs += m > 0;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    live_seqs = __reduce_add_sync(0xffffffffu, live_seqs);
+  }
   // dB / (S' N) (1 / (k N)) (c E - k N): the integer part is exact.
   const float db = p.d_balance && ns > 0 ? __ldg(p.d_balance) / ((float)live_seqs * (float)ns) : 0.f;
   const float dz = p.d_z && all > 0 ? 2.f * __ldg(p.d_z) / (float)all : 0.f;
   float f[V];
-  const float kn = (float)((int64_t)k * (ns > 0 ? ns : 1));
+  const float kn = db / (float)((int64_t)k * (ns > 0 ? ns : 1));
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    f[i] = e0 + i < E ? (float)((int64_t)__ldg(p.counts + seq * E + e0 + i) * E - (int64_t)k * ns) / kn : 0.f;
+    f[i] = e0 + i < E ? (float)((int64_t)__ldg(p.counts + seq * E + e0 + i) * E - (int64_t)k * ns) * kn : 0.f;
 
   for (int64_t base = lo + warp * TPW; base < hi; base += kRouteWarps * TPW) {
     const int64_t t = base + lane / G;
@@ -494,84 +710,95 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
     const bool live = inside && (!p.mask || __ldg(p.mask + t));
     float v[V];
     row_load<V>(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
-    float mx = v[0];
+    // The weights' part per slot.
+    int id[KS];
+    float g[KS], w[KS], dot = 0.f;
+    if (p.d_weights) {
 #pragma unroll
-    for (int i = 1; i < V; ++i) mx = fmaxf(mx, v[i]);
-    mx = group_max<G>(mx);
-    const bool keep = mx > -INFINITY;
-    float d[V], slope[V];
-    // Softmax part: p, and with softmax scoring q = p.
-    float total = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      d[i] = keep && e0 + i < E ? expf(v[i] - mx) : 0.f;
-      total += d[i];
+      for (int s = 0; s < KS; ++s) {
+        const int j = s * G + gl;
+        id[s] = live && j < k ? __ldg(p.ids + t * k + j) : -1;
+        if (id[s] >= E) id[s] = -1;
+        w[s] = id[s] >= 0 ? __ldg(p.weights + t * k + j) : 0.f;
+        g[s] = id[s] >= 0 ? __ldg(p.d_weights + t * k + j) : 0.f;
+        dot = fmaf(w[s], g[s], dot);
+      }
     }
-    total = group_sum<G>(total);
-    const float inv = keep ? 1.f / total : 0.f;
-    const float zl = keep ? dz * (mx + logf(total)) : 0.f;
-    // <dw, w> over the slots in use.
-    float dot = 0.f;
-    if (p.d_weights && inside) {
-      for (int j = 0; j < k; ++j)
-        if (__ldg(p.ids + t * k + j) >= 0) dot += __ldg(p.d_weights + t * k + j) * __ldg(p.weights + t * k + j);
+    const float mx = group_max<G>(lane_max(v));
+    const bool keep = mx > -INFINITY;
+    const float mxl = keep ? mx * kLog2e : 0.f;
+    float d[V];
+    float total = row_exp(v, mxl, d);
+    if (p.d_weights) {
+      dot = group_sum<G>(dot);
+      const float off = p.normalize ? dot : 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        g[s] = w[s] * (g[s] - off);
+        if (p.sigmoid && id[s] >= 0)  // 1 - sigmoid, from the slot's own logit
+          g[s] *= rcp_ftz(1.f + ex2_ftz(elem_load(p.logits, p.type, t * p.ld + id[s]) * kLog2e));
+        // Slots of one expert (the caller's choice may repeat it) are added
+        // in slot order by the lowest of their lanes.
+        const int key = id[s] >= 0 ? lane / G * (G * V) + id[s] : -1 - lane;
+        const uint32_t peers = __match_any_sync(0xffffffffu, key);
+        bool mine = true;
+        if (__any_sync(0xffffffffu, peers != 1u << lane)) {
+          float sum = 0.f;
+          for (int l = 0; l < 32; ++l) {
+            const float x = __shfl_sync(0xffffffffu, g[s], l);
+            if (peers >> l & 1u) sum += x;
+          }
+          g[s] = sum;
+          mine = lane == __ffs(peers) - 1;
+        }
+        if (id[s] >= 0 && mine) row[id[s]] += g[s];
+        __syncwarp();
+      }
     }
     if (!p.sigmoid) {
       float fq = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        d[i] *= inv;
-        fq += f[i] * d[i];
-        slope[i] = 1.f;
-      }
+      for (int i = 0; i < V; ++i) fq = fmaf(f[i], d[i], fq);
+      total = group_sum<G>(total);
       fq = group_sum<G>(fq);
-      const float extra = zl - (p.normalize ? 0.f : dot);
+      const float inv = keep ? 1.f / total : 0.f;
+      // A row's share of every p: the z loss, the centring, the weights' dot.
+      const float every = dz * ((mxl + lg2_ftz(total)) * kLn2) - fq * inv - (p.normalize ? 0.f : dot);
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i] *= db * (f[i] - fq) + extra;
+      for (int i = 0; i < V; ++i) d[i] = d[i] * inv * (f[i] + every);
     } else {
-      const SigmoidRow sg(mx);
-      float q[V], norm = 0.f, fq = 0.f;
+      float q[V], ds[V], norm = 0.f, fq = 0.f;
+      row_sigmoid(v, d, mx, mxl, q, ds);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float r = sg.r(v[i]);
-        q[i] = keep && e0 + i < E ? sg.scaled(r) : 0.f;
-        slope[i] = sg.slope(r);
         norm += q[i];
-        fq += f[i] * q[i];
+        fq = fmaf(f[i], q[i], fq);
       }
       norm = group_sum<G>(norm);
       fq = group_sum<G>(fq);
-      const float qi = keep ? 1.f / norm : 0.f;
-      fq *= qi;
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = d[i] * inv * zl + db * (q[i] * qi) * (f[i] - fq) * slope[i];
-    }
-    if (p.d_weights && keep) {
-      const float off = p.normalize ? dot : 0.f;
-      for (int j = 0; j < k; ++j) {
-        const int at = __ldg(p.ids + t * k + j) - e0;
-        if (at < 0 || at >= V) continue;
-        const float g = __ldg(p.weights + t * k + j) * (__ldg(p.d_weights + t * k + j) - off);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i == at) d[i] += g * slope[i];
+      const float qi = keep ? 1.f / norm : 0.f, centre = fq * qi;
+      float zl = 0.f;
+      if (p.d_z) {
+        total = group_sum<G>(total);
+        zl = keep ? dz * ((mxl + lg2_ftz(total)) * kLn2) / total : 0.f;
       }
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = fmaf(ds[i] * qi, f[i] - centre, d[i] * zl);
     }
-    if (!inside) continue;
+    if (p.d_weights) {
 #pragma unroll
-    for (int c = 0; c < V; c += 8) {
-      if (!keep) {
+      for (int i = 0; i < V; ++i) d[i] += row[e0 + i];
+      __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[c + i] = 0.f;
-      }
-      if (p.vec_out) {
-        if (e0 + c < E) elem_store8(p.d_logits, p.type, t * E + e0 + c, d + c);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (e0 + c + i < E) elem_store(p.d_logits, p.type, t * E + e0 + c + i, d[c + i]);
-      }
+      for (int s = 0; s < KS; ++s)
+        if (id[s] >= 0) row[id[s]] = 0.f;
+      __syncwarp();
     }
+    if (!keep) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = 0.f;
+    }
+    if (inside) row_put<V>(p.d_logits, p.type, p.vec_out, t * E, e0, E, d);
   }
 }
 

@@ -161,7 +161,10 @@ def lib() -> ctypes.CDLL:
     f64 = ctypes.c_double
     L.moe_route_train_workspace_size.argtypes = [i64, i32, i64]
     L.moe_route_train_workspace_size.restype = sz
-    L.moe_route_train.argtypes = [vp, i32, i64, i64, i32, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.moe_route_train_counters.argtypes = [i64, i32, i64]
+    L.moe_route_train_counters.restype = i64
+    L.moe_route_train.argtypes = [vp, i32, i64, i64, i32, i32, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp,
+                                  vp]
     L.moe_route_train.restype = ctypes.c_int
     L.moe_route_backward.argtypes = [vp, i32, i64, i64, i32, i32, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     L.moe_route_backward.restype = ctypes.c_int

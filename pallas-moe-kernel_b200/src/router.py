@@ -18,6 +18,7 @@ current stream and never synchronise the host.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -128,6 +129,33 @@ def _call(dev: torch.device, fn, *args) -> None:
             _lib.check(fn(*args, _stream_handle(dev)))
 
 
+_COUNTERS: dict = {}
+
+
+def _stream_counters(dev: torch.device, stream: int, n: int) -> torch.Tensor:
+    """n int32 counters that are zero between the calls of one stream (each
+    call leaves them so); fresh ones for every call that a CUDA graph
+    captures, which sets them to zero at each replay."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.int32, device=dev)
+    c = _COUNTERS.get((dev.index, stream))
+    if c is None or c.numel() < n:
+        c = _COUNTERS[dev.index, stream] = torch.zeros(max(n, 1024), dtype=torch.int32, device=dev)
+    return c
+
+
+_SCALARS: dict = {}
+
+
+def _scalars(dev: torch.device):
+    """An int32 and a float32 scalar on the device, for new_empty: half the
+    host time of torch.empty with its keywords (1.3 against 2.3 us)."""
+    s = _SCALARS.get(dev.index)
+    if s is None:
+        s = _SCALARS[dev.index] = (torch.empty((), dtype=torch.int32, device=dev), torch.empty((), device=dev))
+    return s
+
+
 def _route_args(logits, mask, sequences, scoring):
     """(logits with unit column stride, element type, row stride, mask bytes, scoring code)."""
     if not logits.is_cuda or logits.dim() != 2:
@@ -147,6 +175,13 @@ def _route_args(logits, mask, sequences, scoring):
         _on(logits.device, mask=mask)
         mask = mask.contiguous()
     return logits, code, logits.stride(0) if T > 1 else E, mask, how
+
+
+@functools.lru_cache(maxsize=4096)
+def _route_space(T: int, E: int, sequences: int):
+    """(workspace bytes, counters) of a routing."""
+    L = _lib.lib()
+    return int(L.moe_route_train_workspace_size(T, E, sequences)), int(L.moe_route_train_counters(T, E, sequences))
 
 
 def route_forward_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Tensor] = None,
@@ -179,21 +214,25 @@ def route_forward_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Ten
         if tuple(ids.shape) != (T, k):
             raise ValueError(f"ids is {tuple(ids.shape)}, expected {(T, k)}")
         _on(dev, ids=ids)
+        if ids.dtype.is_floating_point or ids.dtype == torch.bool:
+            raise TypeError(f"ids are {ids.dtype}, not integers")
         ids = ids.to(torch.int32).contiguous()
     if not 1 <= k <= min(16, E) or E > 1024:
         raise ValueError(f"k={k}, E={E}: 1 <= k <= min(16, E) and E <= 1024 are supported")
-    i32 = {"dtype": torch.int32, "device": dev}
-    f32 = {"dtype": torch.float32, "device": dev}
-    out = RouteTrain(torch.empty((T, k), **i32), torch.empty((T, k), **f32), torch.empty((sequences, E), **i32),
-                     torch.empty(sequences, **i32), torch.empty((), **f32), torch.empty((), **f32))
+    i32, f32 = _scalars(dev)
+    o_ids, o_weights, o_counts = i32.new_empty((T, k)), f32.new_empty((T, k)), i32.new_empty((sequences, E))
+    o_tokens, balance, z = i32.new_empty(sequences), torch.empty_like(f32), torch.empty_like(f32)
     L = _lib.lib()
-    need = int(L.moe_route_train_workspace_size(T, E, sequences))
+    need, counters = _route_space(T, E, sequences)
+    stream = _stream_handle(dev)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = _stream_workspace(dev, _stream_handle(dev), need)
+        workspace = _stream_workspace(dev, stream, need)
+    counters = _stream_counters(dev, stream, counters)
     _call(dev, L.moe_route_train, logits.data_ptr(), code, ld, T, E, k, sequences,
           None if mask is None else mask.data_ptr(), None if ids is None else ids.data_ptr(), how, normalize,
-          *(t.data_ptr() for t in out), workspace.data_ptr(), need)
-    return out
+          o_ids.data_ptr(), o_weights.data_ptr(), o_counts.data_ptr(), o_tokens.data_ptr(), balance.data_ptr(),
+          z.data_ptr(), workspace.data_ptr(), need, counters.data_ptr())
+    return RouteTrain(o_ids, o_weights, o_counts, o_tokens, balance, z)
 
 
 def route_backward(logits: torch.Tensor, routed: RouteTrain, *, d_weights: Optional[torch.Tensor] = None,

@@ -125,7 +125,7 @@ def test_route_abi_refusals():
 
     def call(elem=0, ld=8, T=4, E=8, k=2, S=1, scoring=0, logits=p, out=p, ws=p, nbytes=1 << 20):
         return L.moe_route_train(logits, elem, ld, T, E, k, S, None, None, scoring, 1, out, out, out, out, out, out, ws,
-                                 nbytes, None)
+                                 nbytes, p, None)
     assert call(k=0) == call(k=9) == call(k=17, E=64, ld=64) == call(E=1025, ld=1025) == call(T=-1) == -1
     assert call(T=1 << 30, k=2) == -1                                   # T k reaches 2^31
     assert call(S=3) == call(S=0) == call(ld=7) == call(scoring=2) == -1
