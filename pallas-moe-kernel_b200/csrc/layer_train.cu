@@ -3,7 +3,7 @@
 // movement, and gradient norms and clipping.  Declarations:
 // include/moe_b200.h.
 #include <algorithm>
-#include <cstring>
+#include <cstdlib>
 
 #include "abi_util.h"
 #include "grad_norm.cuh"
@@ -17,17 +17,19 @@ static size_t elem_bytes(int type) { return type == MOE_ELEM_F32 ? 4 : 2; }
 static bool elem_ok(int type) { return type == MOE_ELEM_F32 || type == MOE_ELEM_BF16 || type == MOE_ELEM_F16; }
 
 // ------------------------------------------------------------------ routing
-// Lanes per row: 8 experts a lane up to 256 experts (a 16-byte vector of the
-// 16-bit types), then the whole warp with more experts a lane.
+// Lanes per row: 8 experts a lane up to 16 experts, then 16, and the whole
+// warp with 32 above 512.
 static int route_lanes(int E) {
   int g = 1;
-  while (g < 32 && g * 8 < E) g *= 2;
+  while (g < 32 && g * (E <= 16 ? 8 : 16) < E) g *= 2;
   return g;
 }
 
 // Blocks per sequence: enough that a warp has one step of tokens, and at most
-// kRouteBlocks over all sequences where a sequence is longer than that.
-constexpr int64_t kRouteBlocks = 148 * 4;
+// kRouteBlocks over all sequences where a sequence is longer than that (what
+// is resident at 80 registers a thread: a second, short wave costs its whole
+// length).
+constexpr int64_t kRouteBlocks = 148 * 3;
 static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
   const int64_t step = kRouteWarps * (32 / route_lanes(E));
   const int64_t most = std::max<int64_t>(1, kRouteBlocks / std::max<int64_t>(1, sequences));
@@ -189,6 +191,37 @@ static int check_tensors(const moe_tensor_desc* t, int n, int norm_type, bool wi
       return fail(MOE_ERR_MISALIGNED, "tensor %d is not aligned to its elements", i);
   }
   return 0;
+}
+
+// Outputs that share memory would be scaled twice, in an order nobody knows.
+// Dense tensors are compared by their ranges, those of several rows by their
+// first element (rows of two slices of one matrix interleave).  Lists come in
+// the order of their addresses more often than not: that needs no sorting.
+static int check_outputs(const moe_tensor_desc* t, int n) {
+  auto start = [&](int i) { return reinterpret_cast<uintptr_t>(t[i].out); };
+  auto end = [&](int i) { return start(i) + (t[i].rows == 1 ? t[i].cols : 1) * elem_bytes(t[i].out_type); };
+  auto live = [&](int i) { return t[i].rows && t[i].cols; };
+  int last = -1;
+  bool sorted = true, apart = true;
+  for (int i = 0; i < n; ++i) {
+    if (!live(i)) continue;
+    if (last >= 0 && start(i) < end(last)) {
+      sorted = false;
+      break;
+    }
+    last = i;
+  }
+  if (!sorted) {
+    int* order = static_cast<int*>(malloc(sizeof(int) * (size_t)n));
+    if (!order) return fail(MOE_ERR_INVALID_ARG, "no memory for a list of %d tensors", n);
+    int m = 0;
+    for (int i = 0; i < n; ++i)
+      if (live(i)) order[m++] = i;
+    std::sort(order, order + m, [&](int a, int b) { return start(a) < start(b); });
+    for (int i = 1; i < m; ++i) apart = apart && start(order[i]) >= end(order[i - 1]);
+    free(order);
+  }
+  return apart ? 0 : fail(MOE_ERR_INVALID_ARG, "an output is in the list twice, or two of them share memory");
 }
 
 static int entry_head(const GradEntry& e) {
@@ -374,15 +407,15 @@ int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T
   p.sigmoid = scoring == MOE_SCORE_SIGMOID;
   p.normalize = normalize != 0;
   if (E > 512) return launch_route_k<32, 32>(p, blocks, st);
-  if (E > 256) return launch_route_k<32, 16>(p, blocks, st);
+  if (E <= 8) return launch_route_k<1, 8>(p, blocks, st);
+  if (E <= 16) return launch_route_k<2, 8>(p, blocks, st);
   switch (route_lanes(E)) {
-    case 1: return launch_route_k<1, 8>(p, blocks, st);
-    case 2: return launch_route_k<2, 8>(p, blocks, st);
-    case 4: return launch_route_k<4, 8>(p, blocks, st);
-    case 8: return launch_route_k<8, 8>(p, blocks, st);
-    case 16: return launch_route_k<16, 8>(p, blocks, st);
+    case 2: return launch_route_k<2, 16>(p, blocks, st);
+    case 4: return launch_route_k<4, 16>(p, blocks, st);
+    case 8: return launch_route_k<8, 16>(p, blocks, st);
+    case 16: return launch_route_k<16, 16>(p, blocks, st);
   }
-  return launch_route_k<32, 8>(p, blocks, st);
+  return launch_route_k<32, 16>(p, blocks, st);
 }
 
 int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
@@ -423,15 +456,15 @@ int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_
   p.normalize = normalize != 0;
   const int64_t blocks = p.chunks * sequences;
   if (E > 512) return launch_backward_k<32, 32>(p, blocks, st);
-  if (E > 256) return launch_backward_k<32, 16>(p, blocks, st);
+  if (E <= 8) return launch_backward_k<1, 8>(p, blocks, st);
+  if (E <= 16) return launch_backward_k<2, 8>(p, blocks, st);
   switch (route_lanes(E)) {
-    case 1: return launch_backward_k<1, 8>(p, blocks, st);
-    case 2: return launch_backward_k<2, 8>(p, blocks, st);
-    case 4: return launch_backward_k<4, 8>(p, blocks, st);
-    case 8: return launch_backward_k<8, 8>(p, blocks, st);
-    case 16: return launch_backward_k<16, 8>(p, blocks, st);
+    case 2: return launch_backward_k<2, 16>(p, blocks, st);
+    case 4: return launch_backward_k<4, 16>(p, blocks, st);
+    case 8: return launch_backward_k<8, 16>(p, blocks, st);
+    case 16: return launch_backward_k<16, 16>(p, blocks, st);
   }
-  return launch_backward_k<32, 8>(p, blocks, st);
+  return launch_backward_k<32, 16>(p, blocks, st);
 }
 
 // ------------------------------------------------------------------ rows
@@ -511,6 +544,7 @@ int moe_clip_grads(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type,
                    const float* given_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   t_err[0] = 0;
   if (int r = check_tensors(tensors, n, norm_type, true)) return r;
+  if (int r = check_outputs(tensors, n)) return r;
   if (!(max_norm >= 0.0)) return fail(MOE_ERR_INVALID_ARG, "max_norm %g", max_norm);
   if (!given_norm && !norm) return fail(MOE_ERR_INVALID_ARG, "null norm");
   if (!given_norm)

@@ -95,81 +95,96 @@ __device__ __forceinline__ void unpack16(uint32_t u, int type, float& a, float& 
     b = f.y;
   }
 }
-// Eight consecutive elements from a 16-byte aligned address.
-__device__ __forceinline__ void elem_load8(const void* p, int type, int64_t i, float* v) {
-  if (type == kElemF32) {
-    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const float4 a = __ldg(q), b = __ldg(q + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
-    unpack16(a.x, type, v[0], v[1]);
-    unpack16(a.y, type, v[2], v[3]);
-    unpack16(a.z, type, v[4], v[5]);
-    unpack16(a.w, type, v[6], v[7]);
-  }
-}
 __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
-  return (uint32_t)elem_bits16(a, type) | ((uint32_t)elem_bits16(b, type) << 16);
-}
-__device__ __forceinline__ void elem_store8(void* p, int type, int64_t i, const float* v) {
-  if (type == kElemF32) {
-    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-    q[0] = make_float4(v[0], v[1], v[2], v[3]);
-    q[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
-        make_uint4(pack16(v[0], v[1], type), pack16(v[2], v[3], type), pack16(v[4], v[5], type),
-                   pack16(v[6], v[7], type));
-  }
+  uint32_t r;
+  if (type == kElemBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
 }
 __device__ __forceinline__ void elem_store(void* p, int type, int64_t i, float v) {
   if (type == kElemF32) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = elem_bits16(v, type);
 }
 
-// Experts [e0, e0 + V) of the row at element offset `row`; -inf past E.  The
-// types are told apart once per row: a choice inside the conversions costs
-// more than they do.
+// Rows are held as pairs: sm_100 adds and multiplies two f32 at a time.
+template <int V>
+struct Row {
+  float2 p[V / 2];
+};
+
+// Experts [e0, e0 + V) of the row at element offset `row`; -inf past E, and
+// throughout for a row that is not live.  The types are told apart once per
+// row: a choice inside the conversions costs more than they do.
 template <int TYPE, int V>
-__device__ __forceinline__ void row_load_t(const void* p, int vec, int64_t row, int e0, int E, bool live,
-                                           float (&v)[V]) {
+__device__ __forceinline__ void row_load_t(const void* p, int vec, int64_t row, int e0, int E, bool live, Row<V>& v) {
+  if (vec) {
 #pragma unroll
-  for (int c = 0; c < V; c += 8) {
-    if (live && vec && e0 + c < E) {
-      elem_load8(p, TYPE, row + e0 + c, v + c);
-    } else {
+    for (int c = 0; c < V; c += 8) {
+      const bool on = live && e0 + c < E;
+      if (TYPE == kElemF32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + row + e0 + c);
+        float4 a = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), b = a;
+        if (on) a = __ldg(q), b = __ldg(q + 1);
+        v.p[c / 2] = make_float2(a.x, a.y), v.p[c / 2 + 1] = make_float2(a.z, a.w);
+        v.p[c / 2 + 2] = make_float2(b.x, b.y), v.p[c / 2 + 3] = make_float2(b.z, b.w);
+      } else {
+        const uint32_t none = TYPE == kElemBF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf twice
+        uint4 a = make_uint4(none, none, none, none);
+        if (on) a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + row + e0 + c));
+        unpack16(a.x, TYPE, v.p[c / 2].x, v.p[c / 2].y);
+        unpack16(a.y, TYPE, v.p[c / 2 + 1].x, v.p[c / 2 + 1].y);
+        unpack16(a.z, TYPE, v.p[c / 2 + 2].x, v.p[c / 2 + 2].y);
+        unpack16(a.w, TYPE, v.p[c / 2 + 3].x, v.p[c / 2 + 3].y);
+      }
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[c + i] = live && e0 + c + i < E ? elem_load(p, TYPE, row + e0 + c + i) : -INFINITY;
+    for (int i = 0; i < V; ++i) {
+      const float x = live && e0 + i < E ? elem_load(p, TYPE, row + e0 + i) : -INFINITY;
+      (i & 1 ? v.p[i / 2].y : v.p[i / 2].x) = x;
     }
   }
 }
 template <int V>
 __device__ __forceinline__ void row_load(const void* p, int type, int vec, int64_t row, int e0, int E, bool live,
-                                         float (&v)[V]) {
+                                         Row<V>& v) {
   if (type == kElemF32) row_load_t<kElemF32>(p, vec, row, e0, E, live, v);
   else if (type == kElemBF16) row_load_t<kElemBF16>(p, vec, row, e0, E, live, v);
   else row_load_t<kElemF16>(p, vec, row, e0, E, live, v);
 }
 template <int TYPE, int V>
-__device__ __forceinline__ void row_put_t(void* p, int vec, int64_t row, int e0, int E, const float (&v)[V]) {
+__device__ __forceinline__ void row_put_t(void* p, int vec, int64_t row, int e0, int E, const Row<V>& v) {
+  if (vec) {
 #pragma unroll
-  for (int c = 0; c < V; c += 8) {
-    if (vec) {
-      if (e0 + c < E) elem_store8(p, TYPE, row + e0 + c, v + c);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (e0 + c + i < E) elem_store(p, TYPE, row + e0 + c + i, v[c + i]);
+    for (int c = 0; c < V; c += 8) {
+      const float2 *q = v.p + c / 2;
+      if (e0 + c >= E) continue;
+      if (TYPE == kElemF32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + row + e0 + c);
+        d[0] = make_float4(q[0].x, q[0].y, q[1].x, q[1].y);
+        d[1] = make_float4(q[2].x, q[2].y, q[3].x, q[3].y);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + e0 + c) =
+            make_uint4(pack16(q[0].x, q[0].y, TYPE), pack16(q[1].x, q[1].y, TYPE), pack16(q[2].x, q[2].y, TYPE),
+                       pack16(q[3].x, q[3].y, TYPE));
+      }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e0 + i < E) elem_store(p, TYPE, row + e0 + i, i & 1 ? v.p[i / 2].y : v.p[i / 2].x);
   }
 }
 template <int V>
-__device__ __forceinline__ void row_put(void* p, int type, int vec, int64_t row, int e0, int E, const float (&v)[V]) {
+__device__ __forceinline__ void row_put(void* p, int type, int vec, int64_t row, int e0, int E, const Row<V>& v) {
   if (type == kElemF32) row_put_t<kElemF32>(p, vec, row, e0, E, v);
   else if (type == kElemBF16) row_put_t<kElemBF16>(p, vec, row, e0, E, v);
   else row_put_t<kElemF16>(p, vec, row, e0, E, v);
+}
+template <int V>
+__device__ __forceinline__ void row_fill(Row<V>& v, float x) {
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) v.p[i] = make_float2(x, x);
 }
 
 template <int G>
@@ -214,26 +229,28 @@ __device__ __forceinline__ float rcp_ftz(float x) {
 }
 
 template <int V>
-__device__ __forceinline__ float lane_max(const float (&v)[V]) {
-  float m = v[0];
+__device__ __forceinline__ float lane_max(const Row<V>& v) {
+  float m = fmaxf(v.p[0].x, v.p[0].y);
 #pragma unroll
-  for (int i = 1; i < V; ++i) m = fmaxf(m, v[i]);
+  for (int i = 1; i < V / 2; ++i) m = fmaxf(m, fmaxf(v.p[i].x, v.p[i].y));
   return m;
 }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // e_i = 2^(l_i log2 e - mxl), mxl = the row maximum times log2 e, rounded: one
 // factor near 1 in all of them, which the ratios p = e / sum(e) and
 // lse = (mxl + log2 sum(e)) ln 2 are free of.  Rows that are not kept have
 // l = -inf throughout, and e = 0.
 template <int V>
-__device__ __forceinline__ float row_exp(const float (&v)[V], float mxl, float (&e)[V]) {
-  float total = 0.f;
+__device__ __forceinline__ float row_exp(const Row<V>& v, float mxl, Row<V>& e) {
+  float2 total = both(0.f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    e[i] = ex2_ftz(fmaf(v[i], kLog2e, -mxl));
-    total += e[i];
+  for (int i = 0; i < V / 2; ++i) {
+    const float2 x = __ffma2_rn(v.p[i], both(kLog2e), both(-mxl));
+    e.p[i] = make_float2(ex2_ftz(x.x), ex2_ftz(x.y));
+    total = __fadd2_rn(total, e.p[i]);
   }
-  return total;
+  return total.x + total.y;
 }
 
 // Sigmoid scores from the same exponentials.  For a maximum mx >= 0,
@@ -241,25 +258,26 @@ __device__ __forceinline__ float row_exp(const float (&v)[V], float mxl, float (
 // s' = s 2^-mxl = e / (e 2^mxl + 1), so that a row of very negative logits has
 // ratios at all.  Both are s' = e t with t = 1 / (e a + b), and 1 - s = b t.
 // Above mx = 40, e would lose scores near 0 logits: they get exponentials of
-// their own.  `ds` receives s' (1 - s), the derivative.
-template <int V>
-__device__ __forceinline__ void row_sigmoid(const float (&v)[V], const float (&e)[V], float mx, float mxl,
-                                            float (&s)[V], float (&ds)[V]) {
+// their own.  f(i, s', s' (1 - s)) takes a pair at a time.
+template <int V, class F>
+__device__ __forceinline__ void row_sigmoid(const Row<V>& v, const Row<V>& e, float mx, float mxl, F&& f) {
   if (mx > 40.f) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float r = ex2_ftz(-kLog2e * v[i]);
-      s[i] = rcp_ftz(1.f + r);
-      ds[i] = r > 1e18f ? s[i] : r * s[i] * s[i];
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 r = make_float2(ex2_ftz(-kLog2e * v.p[i].x), ex2_ftz(-kLog2e * v.p[i].y));
+      const float2 s = make_float2(rcp_ftz(1.f + r.x), rcp_ftz(1.f + r.y));
+      f(i, s, make_float2(r.x > 1e18f ? s.x : r.x * s.x * s.x, r.y > 1e18f ? s.y : r.y * s.y * s.y));
     }
     return;
   }
-  const float a = mx >= 0.f ? 1.f : ex2_ftz(mxl), b = mx >= 0.f ? ex2_ftz(-mxl) : 1.f;
+  const float other = ex2_ftz(-fabsf(mxl));
+  const float2 a = both(mx >= 0.f ? 1.f : other), b = both(mx >= 0.f ? other : 1.f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float t = rcp_ftz(fmaf(e[i], a, b));
-    s[i] = e[i] * t;
-    ds[i] = s[i] * (b * t);
+  for (int i = 0; i < V / 2; ++i) {
+    const float2 x = __ffma2_rn(e.p[i], a, b);
+    const float2 t = make_float2(rcp_ftz(x.x), rcp_ftz(x.y));
+    const float2 s = __fmul2_rn(e.p[i], t);
+    f(i, s, __fmul2_rn(s, __fmul2_rn(b, t)));
   }
 }
 
@@ -462,8 +480,14 @@ __device__ __forceinline__ void route_finish(const RouteParams& p, int64_t seq, 
   }
 }
 
+// Blocks per SM that the register budget is cut for.
 template <int G, int V, int KMAX>
-__global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteParams p) {
+constexpr int route_residents() {
+  return V == 32 ? 1 : (KMAX + G - 1) / G <= 4 ? 3 : 2;
+}
+
+template <int G, int V, int KMAX>
+__global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_train_kernel(const RouteParams p) {
   constexpr int TPW = 32 / G;                // tokens per warp and step
   constexpr int KS = (KMAX + G - 1) / G;     // slots per lane
   extern __shared__ int s_cnt[];             // [E] counts, then [warps][G V] sums of q
@@ -484,17 +508,16 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
   const int chunk = blockIdx.x % p.chunks;
   const int64_t lo = seq * p.seq_len + p.seq_len * chunk / p.chunks;
   const int64_t hi = seq * p.seq_len + p.seq_len * (chunk + 1) / p.chunks;
-  float acc[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  Row<V> acc;
+  row_fill(acc, 0.f);
   float z = 0.f;
   int n = 0;
   for (int64_t base = lo + warp * TPW; base < hi; base += kRouteWarps * TPW) {
     const int64_t t = base + lane / G;
     const bool inside = t < hi;
     const bool live = inside && (!p.mask || __ldg(p.mask + t));
-    float v[V];
-    row_load<V>(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
+    Row<V> v;
+    row_load(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
     int id[KS];
     float sel[KS];
     if (p.given) {
@@ -509,36 +532,35 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
     float m = lane_max(v);
     const float mx = group_max<G>(m);
     const bool keep = mx > -INFINITY;
-    if (!keep) {  // a row of NaN takes no part either
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = -INFINITY;
-    }
+    if (!keep) row_fill(v, -INFINITY);  // a row of NaN takes no part either
     const float mxl = keep ? mx * kLog2e : 0.f;
-    float ex[V];
+    Row<V> ex;
     const float total = group_sum<G>(row_exp(v, mxl, ex));
     const float lse = keep ? (mxl + lg2_ftz(total)) * kLn2 : 0.f;
     z += lse * lse;
     n += keep;
     float inv;  // 1 / the sum of the scores
     if (!p.sigmoid) {
-      inv = keep ? 1.f / total : 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(ex[i], inv, acc[i]);
+      inv = keep ? rcp_ftz(total) : 0.f;
     } else {
-      float sc[V], ds[V], sum = 0.f;
-      row_sigmoid(v, ex, mx, mxl, sc, ds);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += sc[i];
-      sum = group_sum<G>(sum);
-      inv = keep ? 1.f / sum : 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(sc[i], inv, acc[i]);
+      float2 sum = both(0.f);
+      row_sigmoid(v, ex, mx, mxl, [&](int i, float2 s, float2) {
+        ex.p[i] = s;
+        sum = __fadd2_rn(sum, s);
+      });
+      const float norm = group_sum<G>(sum.x + sum.y);  // by every lane: other rows of the warp may be kept
+      inv = keep ? rcp_ftz(norm) : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) acc.p[i] = __ffma2_rn(ex.p[i], both(inv), acc.p[i]);
 
     // Choice: k rounds of the row's maximum.
     if (!p.given) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = v[i] > -INFINITY ? v[i] : -INFINITY;  // NaN is never chosen
+      for (int i = 0; i < V / 2; ++i) {  // NaN is never chosen
+        v.p[i].x = v.p[i].x > -INFINITY ? v.p[i].x : -INFINITY;
+        v.p[i].y = v.p[i].y > -INFINITY ? v.p[i].y : -INFINITY;
+      }
       m = lane_max(v);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -554,11 +576,15 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
         int at = -1;
         if (lane == owner) {
 #pragma unroll
-          for (int i = V - 1; i >= 0; --i)
-            if (v[i] == M) at = i;
+          for (int i = V / 2 - 1; i >= 0; --i) {
+            if (v.p[i].y == M) at = 2 * i + 1;
+            if (v.p[i].x == M) at = 2 * i;
+          }
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (i == at) v[i] = -INFINITY;
+          for (int i = 0; i < V / 2; ++i) {
+            if (2 * i == at) v.p[i].x = -INFINITY;
+            if (2 * i + 1 == at) v.p[i].y = -INFINITY;
+          }
           m = lane_max(v);
           at += e0;
         }
@@ -589,7 +615,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
     float scale = p.sigmoid ? ex2_ftz(fminf(mx, 0.f) * kLog2e) : inv;
     if (p.normalize) {
       sum = group_sum<G>(sum);
-      scale = sum == 0.f ? 0.f : 1.f / sum;
+      scale = sum == 0.f ? 0.f : rcp_ftz(sum);
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -607,14 +633,20 @@ __global__ void __launch_bounds__(kRouteThreads) route_train_kernel(const RouteP
 #pragma unroll
   for (int o = G; o < 32; o <<= 1) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    for (int i = 0; i < V / 2; ++i) {
+      acc.p[i].x += __shfl_xor_sync(0xffffffffu, acc.p[i].x, o);
+      acc.p[i].y += __shfl_xor_sync(0xffffffffu, acc.p[i].y, o);
+    }
     z += __shfl_xor_sync(0xffffffffu, z, o);
     n += __shfl_xor_sync(0xffffffffu, n, o);
   }
   float* s_q = reinterpret_cast<float*>(s_cnt + E);
   if (lane < G) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_q[warp * (G * V) + e0 + i] = acc[i];
+    for (int i = 0; i < V / 2; ++i) {
+      s_q[warp * (G * V) + e0 + 2 * i] = acc.p[i].x;
+      s_q[warp * (G * V) + e0 + 2 * i + 1] = acc.p[i].y;
+    }
   }
   if (lane == 0) {
     s_z[warp] = z;
@@ -666,7 +698,7 @@ struct RouteBackward {
 // row in shared memory that is zero between uses (a register exchange takes
 // k V compares a lane).
 template <int G, int V, int KMAX>
-__global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteBackward p) {
+__global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_backward_kernel(const RouteBackward p) {
   constexpr int TPW = 32 / G;
   constexpr int KS = (KMAX + G - 1) / G;
   __shared__ __align__(16) float s_row[kRouteWarps][32 * V];
@@ -695,21 +727,26 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
     all = __reduce_add_sync(0xffffffffu, all);
     live_seqs = __reduce_add_sync(0xffffffffu, live_seqs);
   }
-  // dB / (S' N) (1 / (k N)) (c E - k N): the integer part is exact.
+  // dB / (S' N) (1 / (k N)) (c E - k N): the integer part is exact (in 32 bits
+  // where k N E, which bounds c E, fits).
   const float db = p.d_balance && ns > 0 ? __ldg(p.d_balance) / ((float)live_seqs * (float)ns) : 0.f;
   const float dz = p.d_z && all > 0 ? 2.f * __ldg(p.d_z) / (float)all : 0.f;
-  float f[V];
+  Row<V> f;
   const float kn = db / (float)((int64_t)k * (ns > 0 ? ns : 1));
+  const bool narrow = (int64_t)k * ns * E < (int64_t)1 << 31;
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    f[i] = e0 + i < E ? (float)((int64_t)__ldg(p.counts + seq * E + e0 + i) * E - (int64_t)k * ns) * kn : 0.f;
+  for (int i = 0; i < V; ++i) {
+    const int c = e0 + i < E ? __ldg(p.counts + seq * E + e0 + i) : 0;
+    const float x = narrow ? (float)(c * E - k * ns) : (float)((int64_t)c * E - (int64_t)k * ns);
+    (i & 1 ? f.p[i / 2].y : f.p[i / 2].x) = e0 + i < E ? x * kn : 0.f;
+  }
 
   for (int64_t base = lo + warp * TPW; base < hi; base += kRouteWarps * TPW) {
     const int64_t t = base + lane / G;
     const bool inside = t < hi;
     const bool live = inside && (!p.mask || __ldg(p.mask + t));
-    float v[V];
-    row_load<V>(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
+    Row<V> v;
+    row_load(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
     // The weights' part per slot.
     int id[KS];
     float g[KS], w[KS], dot = 0.f;
@@ -727,7 +764,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
     const float mx = group_max<G>(lane_max(v));
     const bool keep = mx > -INFINITY;
     const float mxl = keep ? mx * kLog2e : 0.f;
-    float d[V];
+    Row<V> d;
     float total = row_exp(v, mxl, d);
     if (p.d_weights) {
       dot = group_sum<G>(dot);
@@ -756,49 +793,48 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
       }
     }
     if (!p.sigmoid) {
-      float fq = 0.f;
+      float2 fs = both(0.f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) fq = fmaf(f[i], d[i], fq);
+      for (int i = 0; i < V / 2; ++i) fs = __ffma2_rn(f.p[i], d.p[i], fs);
       total = group_sum<G>(total);
-      fq = group_sum<G>(fq);
-      const float inv = keep ? 1.f / total : 0.f;
+      const float fq = group_sum<G>(fs.x + fs.y);
+      const float inv = keep ? rcp_ftz(total) : 0.f;
       // A row's share of every p: the z loss, the centring, the weights' dot.
       const float every = dz * ((mxl + lg2_ftz(total)) * kLn2) - fq * inv - (p.normalize ? 0.f : dot);
+      const float2 x = both(inv), y = both(every * inv);
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = d[i] * inv * (f[i] + every);
+      for (int i = 0; i < V / 2; ++i) d.p[i] = __fmul2_rn(d.p[i], __ffma2_rn(f.p[i], x, y));
     } else {
-      float q[V], ds[V], norm = 0.f, fq = 0.f;
-      row_sigmoid(v, d, mx, mxl, q, ds);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        norm += q[i];
-        fq = fmaf(f[i], q[i], fq);
-      }
-      norm = group_sum<G>(norm);
-      fq = group_sum<G>(fq);
-      const float qi = keep ? 1.f / norm : 0.f, centre = fq * qi;
+      Row<V> ds;
+      float2 ns2 = both(0.f), fs = both(0.f);
+      row_sigmoid(v, d, mx, mxl, [&](int i, float2 s, float2 slope) {
+        ns2 = __fadd2_rn(ns2, s);
+        fs = __ffma2_rn(f.p[i], s, fs);
+        ds.p[i] = slope;
+      });
+      const float norm = group_sum<G>(ns2.x + ns2.y), fq = group_sum<G>(fs.x + fs.y);
+      const float qi = keep ? rcp_ftz(norm) : 0.f;
       float zl = 0.f;
       if (p.d_z) {
         total = group_sum<G>(total);
-        zl = keep ? dz * ((mxl + lg2_ftz(total)) * kLn2) / total : 0.f;
+        zl = keep ? dz * ((mxl + lg2_ftz(total)) * kLn2) * rcp_ftz(total) : 0.f;
       }
+      const float2 x = both(qi), y = both(-fq * qi * qi), w2 = both(zl);
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = fmaf(ds[i] * qi, f[i] - centre, d[i] * zl);
+      for (int i = 0; i < V / 2; ++i)
+        d.p[i] = __ffma2_rn(ds.p[i], __ffma2_rn(f.p[i], x, y), __fmul2_rn(d.p[i], w2));
     }
     if (p.d_weights) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i] += row[e0 + i];
+      for (int i = 0; i < V / 2; ++i) d.p[i] = __fadd2_rn(d.p[i], reinterpret_cast<const float2*>(row + e0)[i]);
       __syncwarp();
 #pragma unroll
       for (int s = 0; s < KS; ++s)
         if (id[s] >= 0) row[id[s]] = 0.f;
       __syncwarp();
     }
-    if (!keep) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = 0.f;
-    }
-    if (inside) row_put<V>(p.d_logits, p.type, p.vec_out, t * E, e0, E, d);
+    if (!keep) row_fill(d, 0.f);
+    if (inside) row_put(p.d_logits, p.type, p.vec_out, t * E, e0, E, d);
   }
 }
 

@@ -18,24 +18,26 @@ norm comes back as a device scalar.
 
 from __future__ import annotations
 
+import functools
 import math
 import operator
+import struct
+from array import array
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
 from .kernel import _stream_handle, _stream_workspace
-from .router import _ELEMS, _call
+from .router import _ELEMS, _call, _scalars
 
 __all__ = ["grad_norm", "clip_grads", "clip_grad_norm"]
 
 _NORMS = {1.0: _lib.MOE_NORM_L1, 2.0: _lib.MOE_NORM_L2, math.inf: _lib.MOE_NORM_INF}
 
-# moe_tensor_desc of include/moe_b200.h.
-_DESC = np.dtype([("in", np.uint64), ("out", np.uint64), ("rows", np.int64), ("cols", np.int64), ("in_ld", np.int64),
-                  ("out_ld", np.int64), ("in_type", np.int32), ("out_type", np.int32)])
+# moe_tensor_desc of include/moe_b200.h as 64-bit words: in, out, rows, cols,
+# in_ld, out_ld, and the two element types in one.
+_WORDS = 7
 
 _ptrs = torch.Tensor.data_ptr
 _numel = torch.Tensor.numel
@@ -61,63 +63,73 @@ def _rows_of(t: torch.Tensor):
     return None if dims or ld < cols else (rows, cols, ld)
 
 
+def _column(f, tensors) -> array:
+    """f of every tensor as 64-bit words (array's own constructor takes twice as long from a list of ints)."""
+    return array("q", struct.pack(f"{len(tensors)}q", *map(f, tensors)))
+
+
+def _types(tensors) -> array:
+    kinds = set(map(_dtype, tensors))
+    if not kinds <= _ELEMS.keys():
+        raise TypeError(f"gradients are float32, bfloat16 or float16, not {(kinds - _ELEMS.keys()).pop()}")
+    if len(kinds) == 1:
+        return array("q", [_ELEMS[kinds.pop()]]) * len(tensors)
+    return array("q", [_ELEMS[t.dtype] for t in tensors])
+
+
 def _describe(grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]]):
-    """(descriptors, device) of the list; ``out`` None: the tensors themselves."""
+    """(descriptors, device) of the list; ``out`` None: the tensors themselves.
+    Whole columns at a time: at hundreds of tensors this is the call's cost."""
     grads = list(grads)
     n = len(grads)
     outs = grads if out is None else list(out)
     if len(outs) != n:
         raise ValueError(f"{n} gradients and {len(outs)} outputs")
-    d = np.zeros(n, _DESC)
     if n == 0:
-        return d, None
-    devices = set(map(_device, grads)) | set(map(_device, outs))
+        return array("q"), None
+    devices = set(map(_device, grads))
+    if outs is not grads:
+        devices.update(map(_device, outs))
     if len(devices) > 1 or -1 in devices:
         raise ValueError("gradients and outputs must be CUDA tensors on one device")
-    sides = [("in", grads)] if outs is grads else [("in", grads), ("out", outs)]
-    for side, tensors in sides:
-        d[side] = list(map(_ptrs, tensors))
-        types = set(map(_dtype, tensors))
-        if not types <= _ELEMS.keys():
-            raise TypeError(f"gradients are float32, bfloat16 or float16, not {types - _ELEMS.keys()}")
-        d[side + "_type"] = _ELEMS[types.pop()] if len(types) == 1 else [_ELEMS[t.dtype] for t in tensors]
-    d["rows"] = 1
-    d["cols"] = list(map(_numel, grads))
-    if outs is not grads and [*map(operator.attrgetter("shape"), grads)] != [*map(operator.attrgetter("shape"), outs)]:
-        raise ValueError("an output has another shape than its gradient")
-    if not (all(map(_dense, grads)) and (outs is grads or all(map(_dense, outs)))):
+    d = array("q", bytes(8 * _WORDS * n))
+    d[0::_WORDS] = d[1::_WORDS] = _column(_ptrs, grads)
+    d[2::_WORDS] = array("q", [1]) * n
+    d[3::_WORDS] = numel = _column(_numel, grads)
+    types = outer = _types(grads)
+    if outs is not grads:
+        d[1::_WORDS] = _column(_ptrs, outs)
+        outer = _types(outs)
+        if numel != _column(_numel, outs):
+            raise ValueError("an output has another shape than its gradient")
+    if types.count(types[0]) == n == outer.count(outer[0]):
+        d[6::_WORDS] = array("q", [types[0] | outer[0] << 32]) * n
+    else:
+        d[6::_WORDS] = array("q", [t | u << 32 for t, u in zip(types, outer)])
+    if not all(map(_dense, grads)) or not (outs is grads or all(map(_dense, outs))):
         for i, (g, o) in enumerate(zip(grads, outs)):
-            if g.is_contiguous() and o.is_contiguous():
-                continue
-            if o is not g and g.stride() != o.stride():
-                # Another order of the elements in memory; two row strides of
-                # one order are fine.
-                dims = [x for x in range(g.dim()) if g.shape[x] > 1]
-                same = sorted(dims, key=g.stride) == sorted(dims, key=o.stride)
-            else:
-                same = True
-            rg, ro = _rows_of(g), _rows_of(o)
-            if not same or rg is None or ro is None or (rg[:2] != ro[:2] and 1 not in (rg[0], ro[0])):
-                raise ValueError(f"tensor {i}: strides {g.stride()} and {o.stride()} of shape {tuple(g.shape)} are not "
-                                 "equally spaced rows of one order")
-            if rg[0] == 1 and ro[0] > 1:
-                rg = (ro[0], ro[1], ro[1])
-            elif ro[0] == 1 and rg[0] > 1:
-                ro = (rg[0], rg[1], rg[1])
-            d[i]["rows"], d[i]["cols"], d[i]["in_ld"], d[i]["out_ld"] = rg[0], rg[1], rg[2], ro[2]
-    if outs is grads:
-        d["out"], d["out_type"] = d["in"], d["in_type"]
+            if not (g.is_contiguous() and o.is_contiguous()):
+                d[_WORDS * i + 2:_WORDS * i + 6] = array("q", _strided(i, g, o))
     return d, grads[0].device
 
 
-def _refuse_overlap(d) -> None:
-    """Dense outputs that share memory would be scaled twice."""
-    live = d[(d["rows"] * d["cols"]) > 0]
-    order = np.argsort(live["out"], kind="stable")
-    start = live["out"][order].astype(np.int64)
-    size = np.where(live["rows"] == 1, live["cols"], 1)[order] * np.where(live["out_type"] == 0, 4, 2)[order]
-    if np.any(start[1:] < start[:-1] + size[:-1]):
-        raise ValueError("a tensor is in the list twice, or two of them share memory")
+def _strided(i: int, g: torch.Tensor, o: torch.Tensor):
+    """rows, cols and the two row strides of a pair that is not contiguous."""
+    if g.shape != o.shape:
+        raise ValueError(f"tensor {i}: an output of another shape than its gradient, {tuple(g.shape)}, {tuple(o.shape)}")
+    # The elements' order in memory must be the same; the distance of the rows
+    # may differ.
+    dims = [x for x in range(g.dim()) if g.shape[x] > 1]
+    rg, ro = _rows_of(g), _rows_of(o)
+    if rg is not None and ro is not None and sorted(dims, key=g.stride) == sorted(dims, key=o.stride):
+        if rg[0] == 1:
+            rg = (ro[0], ro[1], ro[1])
+        if ro[0] == 1:
+            ro = (rg[0], rg[1], rg[1])
+        if rg[:2] == ro[:2]:
+            return rg[0], rg[1], rg[2], ro[2]
+    raise ValueError(f"tensor {i}: strides {g.stride()} and {o.stride()} of shape {tuple(g.shape)} are not equally "
+                     "spaced rows of one order")
 
 
 def _norm_code(norm_type) -> int:
@@ -127,8 +139,13 @@ def _norm_code(norm_type) -> int:
     return code
 
 
+@functools.lru_cache(maxsize=4096)
+def _space_bytes(n: int) -> int:
+    return int(_lib.lib().moe_grad_norm_workspace_size(n))
+
+
 def _space(dev, n: int):
-    need = int(_lib.lib().moe_grad_norm_workspace_size(n))
+    need = _space_bytes(n)
     return _stream_workspace(dev, _stream_handle(dev), need), need
 
 
@@ -144,9 +161,9 @@ def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Te
     d, dev = _describe(grads, None)
     if dev is None:
         return torch.zeros((), dtype=torch.float32, device="cuda")
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws, need = _space(dev, len(d))
-    _call(dev, _lib.lib().moe_grad_norm, d.ctypes.data, len(d), code, norm.data_ptr(), ws.data_ptr(), need)
+    norm = torch.empty_like(_scalars(dev)[1])
+    ws, need = _space(dev, len(d) // _WORDS)
+    _call(dev, _lib.lib().moe_grad_norm, d.buffer_info()[0], len(d) // _WORDS, code, norm.data_ptr(), ws.data_ptr(), need)
     return norm
 
 
@@ -157,15 +174,15 @@ def _clip(grads, max_norm, code, given, out):
     d, dev = _describe(grads, out)
     if dev is None:
         return given if given is not None else torch.zeros((), dtype=torch.float32, device="cuda")
-    _refuse_overlap(d)
+    n, at = len(d) // _WORDS, d.buffer_info()[0]
     if given is not None:
         if given.device != dev or given.dtype != torch.float32 or given.numel() != 1:
             raise ValueError("total_norm must be a float32 scalar tensor on the gradients' device")
-        _call(dev, _lib.lib().moe_clip_grads, d.ctypes.data, len(d), code, max_norm, given.data_ptr(), None, None, 0)
+        _call(dev, _lib.lib().moe_clip_grads, at, n, code, max_norm, given.data_ptr(), None, None, 0)
         return given
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws, need = _space(dev, len(d))
-    _call(dev, _lib.lib().moe_clip_grads, d.ctypes.data, len(d), code, max_norm, None, norm.data_ptr(), ws.data_ptr(),
+    norm = torch.empty_like(_scalars(dev)[1])
+    ws, need = _space(dev, len(d) // _WORDS)
+    _call(dev, _lib.lib().moe_clip_grads, at, n, code, max_norm, None, norm.data_ptr(), ws.data_ptr(),
           need)
     return norm
 
@@ -175,7 +192,7 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, norm_type: fl
     """Scales the tensors by ``min(1, max_norm / (norm + 1e-6))`` and returns
     the norm they had (see :func:`grad_norm`).
 
-    In place, or into ``out``: tensors of the same shapes, of any of the three
+    In place, or into ``out``: tensors of the same sizes, of any of the three
     types (one rounding from the f32 product), that share no memory with the
     gradients.  In place nothing is written where the factor is 1.  A NaN norm
     makes every result NaN, as the product says; check the returned norm to

@@ -123,25 +123,32 @@ def _on(dev, **tensors):
 def _call(dev: torch.device, fn, *args) -> None:
     """One library call on ``dev`` and its current stream."""
     if dev.index == torch.cuda.current_device():
-        _lib.check(fn(*args, _stream_handle(dev)))
+        rc = fn(*args, _stream_handle(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.check(fn(*args, _stream_handle(dev)))
+            rc = fn(*args, _stream_handle(dev))
+    if rc:
+        _lib.check(rc)
 
 
 _COUNTERS: dict = {}
 
 
-def _stream_counters(dev: torch.device, stream: int, n: int) -> torch.Tensor:
-    """n int32 counters that are zero between the calls of one stream (each
-    call leaves them so); fresh ones for every call that a CUDA graph
-    captures, which sets them to zero at each replay."""
+def _route_scratch(dev: torch.device, T: int, E: int, sequences: int, workspace: Optional[torch.Tensor]):
+    """(workspace, its bytes, counters) of a routing on the current stream.
+    Counters are zero between the calls of one stream (each call leaves them
+    so); a call that a CUDA graph captures gets fresh ones, set to zero at
+    each replay."""
+    need, n = _route_space(T, E, sequences)
+    stream = _stream_handle(dev)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = _stream_workspace(dev, stream, need)
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=dev)
+        return workspace, need, torch.zeros(n, dtype=torch.int32, device=dev)
     c = _COUNTERS.get((dev.index, stream))
     if c is None or c.numel() < n:
         c = _COUNTERS[dev.index, stream] = torch.zeros(max(n, 1024), dtype=torch.int32, device=dev)
-    return c
+    return workspace, need, c
 
 
 _SCALARS: dict = {}
@@ -157,24 +164,27 @@ def _scalars(dev: torch.device):
 
 
 def _route_args(logits, mask, sequences, scoring):
-    """(logits with unit column stride, element type, row stride, mask bytes, scoring code)."""
+    """(logits with unit column stride, element type, row stride, mask pointer, scoring code, the mask's tensor)."""
     if not logits.is_cuda or logits.dim() != 2:
         raise ValueError("logits must be a 2-D CUDA tensor")
     code = _elem(logits, "logits")
     T, E = logits.shape
-    if E > 1 and logits.stride(1) != 1 or T > 1 and logits.stride(0) < E:
+    ld, col = logits.stride()
+    if E > 1 and col != 1 or T > 1 and ld < E:
         logits = logits.contiguous()
+        ld = E
     if sequences < 1 or T % sequences:
         raise ValueError(f"{T} tokens are not {sequences} sequences of equal length")
     how = _SCORING.get(scoring)
     if how is None:
         raise ValueError(f"scoring {scoring!r} is not 'softmax' or 'sigmoid'")
-    if mask is not None:
-        if mask.dtype != torch.bool or mask.numel() != T:
-            raise ValueError(f"mask must be a bool tensor with one value per token ({T})")
-        _on(logits.device, mask=mask)
-        mask = mask.contiguous()
-    return logits, code, logits.stride(0) if T > 1 else E, mask, how
+    if mask is None:
+        return logits, code, ld if T > 1 else E, None, how, None
+    if mask.dtype != torch.bool or mask.numel() != T:
+        raise ValueError(f"mask must be a bool tensor with one value per token ({T})")
+    _on(logits.device, mask=mask)
+    mask = mask.contiguous()
+    return logits, code, ld if T > 1 else E, mask.data_ptr(), how, mask
 
 
 @functools.lru_cache(maxsize=4096)
@@ -207,7 +217,7 @@ def route_forward_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Ten
     ``permute`` drops the -1 entries and reports them in the device status
     word.  The gradient is :func:`route_backward`; ``train.route_topk_train``
     puts both under autograd."""
-    logits, code, ld, mask, how = _route_args(logits, mask, sequences, scoring)
+    logits, code, ld, mask_ptr, how, mask = _route_args(logits, mask, sequences, scoring)
     dev = logits.device
     T, E = logits.shape
     if ids is not None:
@@ -222,16 +232,11 @@ def route_forward_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Ten
     i32, f32 = _scalars(dev)
     o_ids, o_weights, o_counts = i32.new_empty((T, k)), f32.new_empty((T, k)), i32.new_empty((sequences, E))
     o_tokens, balance, z = i32.new_empty(sequences), torch.empty_like(f32), torch.empty_like(f32)
-    L = _lib.lib()
-    need, counters = _route_space(T, E, sequences)
-    stream = _stream_handle(dev)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = _stream_workspace(dev, stream, need)
-    counters = _stream_counters(dev, stream, counters)
-    _call(dev, L.moe_route_train, logits.data_ptr(), code, ld, T, E, k, sequences,
-          None if mask is None else mask.data_ptr(), None if ids is None else ids.data_ptr(), how, normalize,
-          o_ids.data_ptr(), o_weights.data_ptr(), o_counts.data_ptr(), o_tokens.data_ptr(), balance.data_ptr(),
-          z.data_ptr(), workspace.data_ptr(), need, counters.data_ptr())
+    workspace, need, counters = _route_scratch(dev, T, E, sequences, workspace)
+    _call(dev, _lib.lib().moe_route_train, logits.data_ptr(), code, ld, T, E, k, sequences, mask_ptr,
+          None if ids is None else ids.data_ptr(), how, normalize, o_ids.data_ptr(), o_weights.data_ptr(),
+          o_counts.data_ptr(), o_tokens.data_ptr(), balance.data_ptr(), z.data_ptr(), workspace.data_ptr(), need,
+          counters.data_ptr())
     return RouteTrain(o_ids, o_weights, o_counts, o_tokens, balance, z)
 
 
@@ -243,26 +248,26 @@ def route_backward(logits: torch.Tensor, routed: RouteTrain, *, d_weights: Optio
     gradients of the weights (T, k) and of the two losses (scalars on the
     device); a gradient that is None counts as zero.  ``routed`` is the
     forward's result for the same logits and options."""
-    logits, code, ld, mask, how = _route_args(logits, mask, sequences, scoring)
+    logits, code, ld, mask_ptr, how, mask = _route_args(logits, mask, sequences, scoring)
     dev = logits.device
     T, E = logits.shape
-    k = routed.ids.shape[1]
-    if tuple(routed.ids.shape) != (T, k) or tuple(routed.counts.shape) != (sequences, E):
-        raise ValueError(f"routed has ids {tuple(routed.ids.shape)} and counts {tuple(routed.counts.shape)}, "
-                         f"expected {(T, k)} and {(sequences, E)}")
+    ids, weights, counts, tokens = routed[:4]
+    k = ids.shape[-1]
+    if ids.shape != (T, k) or counts.shape != (sequences, E) or ids.device != dev:
+        raise ValueError(f"routed has ids {tuple(ids.shape)} and counts {tuple(counts.shape)} on {ids.device}, "
+                         f"expected {(T, k)} and {(sequences, E)} on {dev}")
     if d_weights is not None:
-        if tuple(d_weights.shape) != (T, k):
-            raise ValueError(f"d_weights is {tuple(d_weights.shape)}, expected {(T, k)}")
+        if d_weights.shape != (T, k) or d_weights.device != dev:
+            raise ValueError(f"d_weights is {tuple(d_weights.shape)} on {d_weights.device}, expected {(T, k)} on {dev}")
         d_weights = d_weights.to(torch.float32).contiguous()
-    for name, g in (("d_balance", d_balance), ("d_z", d_z)):
-        if g is not None and (g.numel() != 1 or g.dtype != torch.float32):
-            raise ValueError(f"{name} must be a float32 scalar tensor")
-    _on(dev, ids=routed.ids, d_weights=d_weights, d_balance=d_balance, d_z=d_z)
-    d = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _call(dev, _lib.lib().moe_route_backward, logits.data_ptr(), code, ld, T, E, k, sequences, ptr(mask), how,
-          normalize, routed.ids.data_ptr(), routed.weights.data_ptr(), routed.counts.data_ptr(),
-          routed.tokens.data_ptr(), ptr(d_weights), ptr(d_balance), ptr(d_z), d.data_ptr())
+    for g in (d_balance, d_z):
+        if g is not None and (g.numel() != 1 or g.dtype != torch.float32 or g.device != dev):
+            raise ValueError("d_balance and d_z must be float32 scalar tensors on the logits' device")
+    d = logits.new_empty((T, E))
+    _call(dev, _lib.lib().moe_route_backward, logits.data_ptr(), code, ld, T, E, k, sequences, mask_ptr, how,
+          normalize, ids.data_ptr(), weights.data_ptr(), counts.data_ptr(), tokens.data_ptr(),
+          None if d_weights is None else d_weights.data_ptr(), None if d_balance is None else d_balance.data_ptr(),
+          None if d_z is None else d_z.data_ptr(), d.data_ptr())
     return d
 
 
@@ -299,8 +304,8 @@ def combine_rows_backward(dy: torch.Tensor, y_sorted: torch.Tensor, inverse: tor
     _on(dev, y_sorted=y_sorted, inverse=inverse, weights=weights, group_sizes=group_sizes)
     inverse, weights = inverse.contiguous(), weights.to(torch.float32).contiguous()
     gs = group_sizes.to(torch.int32).contiguous()
-    dys = torch.empty((N, D), dtype=dtype, device=dev)
-    dw = torch.empty((T, k), dtype=torch.float32, device=dev)
+    dys = y_sorted.new_empty((N, D), dtype=dtype)
+    dw = weights.new_empty((T, k))
     _call(dev, _lib.lib().moe_combine_rows_backward, dy.data_ptr(), code, y_sorted.data_ptr(), inverse.data_ptr(),
           weights.data_ptr(), gs.data_ptr(), T, k, D, N, gs.numel(), dys.data_ptr(), _ELEMS[dtype], dw.data_ptr())
     return dys, dw
@@ -322,7 +327,7 @@ def gather_rows_backward(dxs: torch.Tensor, inverse: torch.Tensor, *, dtype: Opt
         raise TypeError(f"dtype {dtype} (float32, bfloat16 or float16)")
     _on(dev, inverse=inverse)
     inverse = inverse.contiguous()
-    dx = torch.empty((T, D), dtype=dtype, device=dev)
+    dx = dxs.new_empty((T, D), dtype=dtype)
     _call(dev, _lib.lib().moe_gather_rows_backward, dxs.data_ptr(), code, inverse.data_ptr(), T, k, D, N,
           dx.data_ptr(), _ELEMS[dtype])
     return dx

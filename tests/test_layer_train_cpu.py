@@ -171,7 +171,7 @@ class _Desc(ctypes.Structure):
 def test_gradient_list_abi_refusals():
     L = _lib.lib()
     p = ctypes.c_void_p(256)
-    assert ctypes.sizeof(_Desc) == grads._DESC.itemsize
+    assert ctypes.sizeof(_Desc) == 8 * grads._WORDS
 
     def norm(n=1, kind=2, ws=p, nbytes=1 << 20, **kw):
         d = _Desc(256, 256, 1, 10, 10, 10, 0, 0)
@@ -192,6 +192,12 @@ def test_gradient_list_abi_refusals():
         return L.moe_clip_grads(ctypes.byref(d), 1, 2, max_norm, None, p, p, 1 << 20, None)
     assert clip(-1.0) == clip(math.nan) == clip(out=0) == clip(rows=2, out_ld=3) == -1
     assert clip(out_type=5) == -3 and clip(out=257) == -7
+    def pair(a, b, na, nb):                                        # outputs at a and b, of na and nb f32
+        d = (_Desc * 2)(_Desc(4096, a, 1, na, na, na, 0, 0), _Desc(8192, b, 1, nb, nb, nb, 0, 0))
+        return L.moe_clip_grads(d, 2, 2, 1.0, None, p, p, 8, None)
+    assert pair(256, 256, 1, 1) == pair(256, 260, 2, 1) == pair(260, 256, 1, 2) == -1
+    assert b"share memory" in L.moe_last_error()
+    assert pair(256, 260, 1, 1) == pair(260, 256, 1, 1) == pair(256, 256, 0, 1) == -4      # apart: the workspace is next
     assert L.moe_grad_norm_workspace_size(-1) == 0 and L.moe_grad_norm_workspace_size(1000) > L.moe_grad_norm_workspace_size(1)
 
 
