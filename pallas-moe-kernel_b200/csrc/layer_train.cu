@@ -115,7 +115,10 @@ static int row_threads(int D) { return D >= 1024 ? 256 : D >= 128 ? 32 : 8; }
 
 template <int TPT, int DY, int DYS>
 static int launch_combine(const CombineBwd& p, int zero_blocks, cudaStream_t st) {
-  combine_bwd_kernel<TPT, DY, DYS><<<(unsigned)(p.token_blocks + zero_blocks), kRowThreads, 0, st>>>(p);
+  const unsigned blocks = (unsigned)(p.token_blocks + zero_blocks);
+  if (p.k <= 2) combine_bwd_kernel<TPT, DY, DYS, 2><<<blocks, kRowThreads, 0, st>>>(p);
+  else if (p.k <= 4) combine_bwd_kernel<TPT, DY, DYS, 4><<<blocks, kRowThreads, 0, st>>>(p);
+  else combine_bwd_kernel<TPT, DY, DYS, kRowSlots><<<blocks, kRowThreads, 0, st>>>(p);
   MOE_CUDA_TRY(cudaGetLastError());
   return 0;
 }
@@ -134,12 +137,19 @@ static int launch_combine_t(CombineBwd p, int dy, int dys, int zero_blocks, cuda
   }
   return launch_combine<TPT, 2, 2>(p, zero_blocks, st);
 }
-template <int TPT, int DXS, int DX>
-static int launch_gather(const GatherBwd& p, cudaStream_t st) {
+template <int TPT, int DXS, int DX, int VEC>
+static int launch_gather_v(const GatherBwd& p, cudaStream_t st) {
   const int64_t blocks = (p.T + kRowThreads / TPT - 1) / (kRowThreads / TPT);
-  gather_bwd_kernel<TPT, DXS, DX><<<(unsigned)blocks, kRowThreads, 0, st>>>(p);
+  if (p.k <= 2) gather_bwd_kernel<TPT, DXS, DX, 2, VEC><<<(unsigned)blocks, kRowThreads, 0, st>>>(p);
+  else gather_bwd_kernel<TPT, DXS, DX, kRowSlots, VEC><<<(unsigned)blocks, kRowThreads, 0, st>>>(p);
   MOE_CUDA_TRY(cudaGetLastError());
   return 0;
+}
+template <int TPT, int DXS, int DX>
+static int launch_gather(const GatherBwd& p, cudaStream_t st) {
+  if constexpr (DXS != kElemF32)
+    if (p.D % 8 == 0 && aligned16(p.dxs) && aligned16(p.dx)) return launch_gather_v<TPT, DXS, DX, 8>(p, st);
+  return launch_gather_v<TPT, DXS, DX, 4>(p, st);
 }
 template <int TPT>
 static int launch_gather_t(const GatherBwd& p, int dxs, int dx, cudaStream_t st) {

@@ -187,6 +187,15 @@ __device__ __forceinline__ void row_fill(Row<V>& v, float x) {
   for (int i = 0; i < V / 2; ++i) v.p[i] = make_float2(x, x);
 }
 
+// Brings the next step's row on its way to L1 while this one is computed; it
+// takes no registers, which a load ahead of time would (16 a lane).
+template <int V>
+__device__ __forceinline__ void row_prefetch(const void* p, int type, int64_t row, int e0, int E, bool live) {
+  if (!live || e0 >= E) return;
+  const uint8_t* q = static_cast<const uint8_t*>(p) + (row + e0) * (type == kElemF32 ? 4 : 2);
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
+}
+
 template <int G>
 __device__ __forceinline__ float group_max(float v) {
   if constexpr (G == 32) {
@@ -518,6 +527,8 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     const bool live = inside && (!p.mask || __ldg(p.mask + t));
     Row<V> v;
     row_load(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
+    const int64_t next = t + kRouteWarps * TPW;
+    row_prefetch<V>(p.logits, p.type, next * p.ld, e0, E, next < hi);
     int id[KS];
     float sel[KS];
     if (p.given) {
@@ -747,6 +758,8 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     const bool live = inside && (!p.mask || __ldg(p.mask + t));
     Row<V> v;
     row_load(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
+    const int64_t next = t + kRouteWarps * TPW;
+    row_prefetch<V>(p.logits, p.type, next * p.ld, e0, E, next < hi);
     // The weights' part per slot.
     int id[KS];
     float g[KS], w[KS], dot = 0.f;
@@ -754,10 +767,17 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int j = s * G + gl;
-        id[s] = live && j < k ? __ldg(p.ids + t * k + j) : -1;
-        if (id[s] >= E) id[s] = -1;
-        w[s] = id[s] >= 0 ? __ldg(p.weights + t * k + j) : 0.f;
-        g[s] = id[s] >= 0 ? __ldg(p.d_weights + t * k + j) : 0.f;
+        const bool on = live && j < k;  // the three loads do not wait for one another
+        id[s] = on ? __ldg(p.ids + t * k + j) : -1;
+        w[s] = on ? __ldg(p.weights + t * k + j) : 0.f;
+        g[s] = on ? __ldg(p.d_weights + t * k + j) : 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if (id[s] < 0 || id[s] >= E) {  // dropped, whatever its gradient holds
+          id[s] = -1;
+          w[s] = g[s] = 0.f;
+        }
         dot = fmaf(w[s], g[s], dot);
       }
     }

@@ -20,7 +20,7 @@
 namespace moe {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowSlots = 8;  // slots whose rows are in flight together
+constexpr int kRowSlots = 8;  // vectors of expert rows in flight per thread: 8 slots, or fewer with more vectors each
 
 template <int TYPE>
 __device__ __forceinline__ float4 row_load4(const void* p, int64_t i4) {
@@ -67,8 +67,9 @@ __device__ __forceinline__ float token_sum(float v, float* s_w) {
   return v;
 }
 
-template <int TPT, int DY, int DYS>
+template <int TPT, int DY, int DYS, int SLOTS>
 __global__ void __launch_bounds__(kRowThreads) combine_bwd_kernel(const CombineBwd p) {
+  constexpr int U = kRowSlots / SLOTS;
   __shared__ float s_w[kRowThreads / 32];
   const int n4 = p.D >> 2;
   if (blockIdx.x >= p.token_blocks) {
@@ -94,32 +95,42 @@ __global__ void __launch_bounds__(kRowThreads) combine_bwd_kernel(const CombineB
   const int k = p.k, me = threadIdx.x % TPT;
   const int64_t t = (int64_t)blockIdx.x * (kRowThreads / TPT) + threadIdx.x / TPT;
   const bool inside = t < p.T;
-  for (int j0 = 0; j0 < k; j0 += kRowSlots) {
-    int64_t row[kRowSlots];
-    float w[kRowSlots], dot[kRowSlots];
+  for (int j0 = 0; j0 < k; j0 += SLOTS) {
+    int64_t row[SLOTS];
+    float w[SLOTS], dot[SLOTS];
 #pragma unroll
-    for (int j = 0; j < kRowSlots; ++j) {
+    for (int j = 0; j < SLOTS; ++j) {
       const bool on = inside && j0 + j < k;
       const int r = on ? __ldg(p.inverse + t * k + j0 + j) : -1;
       row[j] = r >= 0 && r < p.rows ? (int64_t)r * n4 : -1;
       w[j] = row[j] >= 0 ? __ldg(p.weights + t * k + j0 + j) : 0.f;
       dot[j] = 0.f;
     }
-    for (int c = me; c < n4; c += TPT) {
-      const float4 g = inside ? row_load4<DY>(p.dy, t * n4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      float4 y[kRowSlots];
+    for (int c0 = me; inside && c0 < n4; c0 += U * TPT) {
+      float4 g[U], y[SLOTS][U];
 #pragma unroll
-      for (int j = 0; j < kRowSlots; ++j)
-        if (row[j] >= 0) y[j] = row_load4<kElemF32>(p.y_sorted, row[j] + c);
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * TPT < n4) g[u] = row_load4<DY>(p.dy, t * n4 + c0 + u * TPT);
 #pragma unroll
-      for (int j = 0; j < kRowSlots; ++j) {
+      for (int j = 0; j < SLOTS; ++j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (row[j] >= 0 && c0 + u * TPT < n4) y[j][u] = row_load4<kElemF32>(p.y_sorted, row[j] + c0 + u * TPT);
+      }
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j) {
         if (row[j] < 0) continue;
-        dot[j] += g.x * y[j].x + g.y * y[j].y + (g.z * y[j].z + g.w * y[j].w);
-        row_store4<DYS>(p.dys, row[j] + c, make_float4(w[j] * g.x, w[j] * g.y, w[j] * g.z, w[j] * g.w));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (c0 + u * TPT >= n4) continue;
+          dot[j] += g[u].x * y[j][u].x + g[u].y * y[j][u].y + (g[u].z * y[j][u].z + g[u].w * y[j][u].w);
+          row_store4<DYS>(p.dys, row[j] + c0 + u * TPT,
+                          make_float4(w[j] * g[u].x, w[j] * g[u].y, w[j] * g[u].z, w[j] * g[u].w));
+        }
       }
     }
 #pragma unroll
-    for (int j = 0; j < kRowSlots; ++j) {
+    for (int j = 0; j < SLOTS; ++j) {
       if (j0 + j >= k) break;
       const float sum = token_sum<TPT>(dot[j], s_w);
       if (inside && me == 0) p.dw[t * k + j0 + j] = sum;
@@ -135,29 +146,77 @@ struct GatherBwd {
   int32_t k, D;
 };
 
-template <int TPT, int DXS, int DX>
+// VEC elements of a row, as they are in memory until they are added: 4, or 8
+// of the 16-bit types where rows allow 16-byte loads (8-byte loads ran the
+// bf16 gather at k = 8, D = 7168 at 5.3 TB/s, these at 6.5).
+template <int TYPE, int VEC>
+struct RawVec {
+  uint4 r;
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if (TYPE == kElemF32 || VEC == 8) {
+      r = __ldg(static_cast<const uint4*>(p) + i);
+    } else {
+      const uint2 u = __ldg(static_cast<const uint2*>(p) + i);
+      r = make_uint4(u.x, u.y, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void add_to(float (&acc)[VEC]) const {
+    float v[8];
+    if (TYPE == kElemF32) {
+      v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
+    } else {
+      unpack16(r.x, TYPE, v[0], v[1]);
+      unpack16(r.y, TYPE, v[2], v[3]);
+      unpack16(r.z, TYPE, v[4], v[5]);
+      unpack16(r.w, TYPE, v[6], v[7]);
+    }
+#pragma unroll
+    for (int x = 0; x < VEC; ++x) acc[x] += v[x];
+  }
+};
+template <int TYPE, int VEC>
+__device__ __forceinline__ void vec_store(void* p, int64_t i, const float (&v)[VEC]) {
+  if (TYPE != kElemF32 && VEC == 8) {
+    static_cast<uint4*>(p)[i] = make_uint4(pack16(v[0], v[1], TYPE), pack16(v[2], v[3], TYPE),
+                                           pack16(v[4 % VEC], v[5 % VEC], TYPE), pack16(v[6 % VEC], v[7 % VEC], TYPE));
+  } else {
+#pragma unroll
+    for (int x = 0; x < VEC; x += 4)
+      row_store4<TYPE>(p, i * (VEC / 4) + x / 4, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
+  }
+}
+
+// SLOTS rows of a token and 8 / SLOTS vectors of each are in flight per thread.
+template <int TPT, int DXS, int DX, int SLOTS, int VEC>
 __global__ void __launch_bounds__(kRowThreads) gather_bwd_kernel(const GatherBwd p) {
-  const int n4 = p.D >> 2, k = p.k, me = threadIdx.x % TPT;
+  constexpr int U = VEC == 8 && SLOTS == 2 ? 2 : kRowSlots / SLOTS;
+  const int n = p.D / VEC, k = p.k, me = threadIdx.x % TPT;
   const int64_t t = (int64_t)blockIdx.x * (kRowThreads / TPT) + threadIdx.x / TPT;
   if (t >= p.T) return;
-  for (int c = me; c < n4; c += TPT) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = 0; j0 < k; j0 += kRowSlots) {
-      float4 v[kRowSlots];
+  for (int c0 = me; c0 < n; c0 += U * TPT) {
+    float acc[U][VEC] = {};
+    for (int j0 = 0; j0 < k; j0 += SLOTS) {
+      RawVec<DXS, VEC> v[SLOTS][U];
 #pragma unroll
-      for (int j = 0; j < kRowSlots; ++j) {
+      for (int j = 0; j < SLOTS; ++j) {
         const int r = j0 + j < k ? __ldg(p.inverse + t * k + j0 + j) : -1;
-        v[j] = r >= 0 && r < p.rows ? row_load4<DXS>(p.dxs, (int64_t)r * n4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool on = r >= 0 && r < p.rows;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (on && c0 + u * TPT < n) v[j][u].load(p.dxs, (int64_t)r * n + c0 + u * TPT);
+          else v[j][u].zero();
+        }
       }
 #pragma unroll
-      for (int j = 0; j < kRowSlots; ++j) {
-        acc.x += v[j].x;
-        acc.y += v[j].y;
-        acc.z += v[j].z;
-        acc.w += v[j].w;
+      for (int j = 0; j < SLOTS; ++j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[j][u].add_to(acc[u]);
       }
     }
-    row_store4<DX>(p.dx, t * n4 + c, acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * TPT < n) vec_store<DX, VEC>(p.dx, t * n + c0 + u * TPT, acc[u]);
   }
 }
 

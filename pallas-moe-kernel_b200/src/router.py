@@ -120,9 +120,15 @@ def _on(dev, **tensors):
             raise ValueError(f"{name} is on {t.device}, the other operands on {dev}")
 
 
+# The calls below cost the host about as much as a small kernel runs: what
+# torch.cuda wraps around these two is a third of a microsecond each.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
 def _call(dev: torch.device, fn, *args) -> None:
     """One library call on ``dev`` and its current stream."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         rc = fn(*args, _stream_handle(dev))
     else:
         with torch.cuda.device(dev):
@@ -140,14 +146,14 @@ def _route_scratch(dev: torch.device, T: int, E: int, sequences: int, workspace:
     so); a call that a CUDA graph captures gets fresh ones, set to zero at
     each replay."""
     need, n = _route_space(T, E, sequences)
-    stream = _stream_handle(dev)
+    key = (dev.index, _stream_handle(dev))
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = _stream_workspace(dev, stream, need)
-    if torch.cuda.is_current_stream_capturing():
+        workspace = _stream_workspace(dev, key[1], need)
+    if _capturing():
         return workspace, need, torch.zeros(n, dtype=torch.int32, device=dev)
-    c = _COUNTERS.get((dev.index, stream))
+    c = _COUNTERS.get(key)
     if c is None or c.numel() < n:
-        c = _COUNTERS[dev.index, stream] = torch.zeros(max(n, 1024), dtype=torch.int32, device=dev)
+        c = _COUNTERS[key] = torch.zeros(max(n, 1024), dtype=torch.int32, device=dev)
     return workspace, need, c
 
 
@@ -276,10 +282,11 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name} must be a 2-D CUDA tensor")
     if t.shape[1] % 4 or t.shape[1] == 0:
         raise ValueError(f"{name} has rows of {t.shape[1]} elements: a positive multiple of 4 is needed")
-    t = t.contiguous()
+    if not t.is_contiguous():
+        return t.contiguous()
     # A contiguous view may start anywhere in its storage; the kernels read
     # four elements at a time.
-    return t if t.data_ptr() % (4 * t.element_size()) == 0 else t.clone()
+    return t.clone() if t.data_ptr() % (4 * t.element_size()) else t
 
 
 def combine_rows_backward(dy: torch.Tensor, y_sorted: torch.Tensor, inverse: torch.Tensor, weights: torch.Tensor,
@@ -295,7 +302,7 @@ def combine_rows_backward(dy: torch.Tensor, y_sorted: torch.Tensor, inverse: tor
     dev = dy.device
     T, k = inverse.shape
     N, D = y_sorted.shape
-    if tuple(dy.shape) != (T, D) or tuple(weights.shape) != (T, k):
+    if dy.shape != (T, D) or weights.shape != (T, k):
         raise ValueError(f"dy {tuple(dy.shape)}, weights {tuple(weights.shape)}: expected {(T, D)} and {(T, k)}")
     if y_sorted.dtype != torch.float32 or inverse.dtype != torch.int32:
         raise TypeError("y_sorted must be float32 and inverse int32")
@@ -304,8 +311,8 @@ def combine_rows_backward(dy: torch.Tensor, y_sorted: torch.Tensor, inverse: tor
     _on(dev, y_sorted=y_sorted, inverse=inverse, weights=weights, group_sizes=group_sizes)
     inverse, weights = inverse.contiguous(), weights.to(torch.float32).contiguous()
     gs = group_sizes.to(torch.int32).contiguous()
-    dys = y_sorted.new_empty((N, D), dtype=dtype)
-    dw = weights.new_empty((T, k))
+    dys = torch.empty_like(y_sorted, dtype=dtype)
+    dw = torch.empty_like(weights)
     _call(dev, _lib.lib().moe_combine_rows_backward, dy.data_ptr(), code, y_sorted.data_ptr(), inverse.data_ptr(),
           weights.data_ptr(), gs.data_ptr(), T, k, D, N, gs.numel(), dys.data_ptr(), _ELEMS[dtype], dw.data_ptr())
     return dys, dw
