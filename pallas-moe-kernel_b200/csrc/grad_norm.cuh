@@ -5,9 +5,9 @@
 //                        writes one f64 partial;
 //   norm_finish_kernel   one block adds the partials in order: the norm (f32);
 //   clip_kernel          out = in * min(1, max_norm / (norm + 1e-6)), rounded
-//                        once to out's type; its blocks add the partials
-//                        themselves, which saves the finish launch.  One
-//                        launch per pair of types in the list.
+//                        once to out's type; on short lists its blocks add
+//                        the partials themselves, which saves the finish
+//                        launch.  One launch per pair of types in the list.
 //
 // HBM-bound: the tensors are read once for the norm and once for the scaling
 // (from L2 where they fit: the scaling walks the units backwards, so that it
@@ -32,7 +32,18 @@ namespace moe {
 constexpr int kNormThreads = 256;
 constexpr int kNormChunks = 8;                          // 16-byte chunks of input a thread has in flight
 constexpr int kNormBlocksPerSm = 4;
-constexpr int kNormMaxBlocks = 148 * kNormBlocksPerSm;  // most blocks (partials) of one launch
+// Blocks of a launch.  Lists of up to kNormLarge units run on the blocks that
+// are resident, and every block of the scaling adds up the partials for
+// itself.  Above that (155 MB of input) a block takes one unit and the hardware
+// hands them out: with resident blocks in a fixed order, the slowest of them
+// set the pace (scaling 2 x 470 M f32 to bf16: 951 us on 592 blocks, 838 on
+// 9472, 798 with one unit each; below, the third launch costs what that
+// gives: 30 M bf16 33 us in two launches and 40 in three, 60 M 64 and 67, 120 M
+// 126 and 123).  A norm's blocks are kept to as many partials
+// as one block then adds up in a few microseconds.
+constexpr int kNormResident = 148 * kNormBlocksPerSm;
+constexpr uint32_t kNormLarge = 8 * kNormResident;
+constexpr int kNormMaxBlocks = 16384;
 
 // Elements of a chunk and of a unit (32 KB of input).
 __host__ __device__ constexpr int chunk_elems(int type) { return type == kElemF32 ? 4 : 8; }
@@ -63,6 +74,18 @@ struct GradList {
 static_assert(sizeof(GradList<kGradSlots>) < 32000, "launch arguments end at 32,764 bytes");
 
 enum : int { kNormL1 = 1, kNormL2 = 2, kNormInf = 3 };
+
+// The tensor that a unit belongs to: the last one whose first unit is not past it.
+template <int SLOTS>
+__device__ __forceinline__ int entry_of(const GradList<SLOTS>& list, uint32_t unit) {
+  int lo = 0, hi = list.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (list.unit0[mid] <= unit) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
 
 // Element i of the tensor (row-major over rows x cols) as an offset.
 __device__ __forceinline__ int64_t entry_at(int64_t i, int64_t rows, int64_t cols, int64_t ld) {
@@ -193,7 +216,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocksPerSm) norm_partial_k
                                                                     double* __restrict__ partial) {
   __shared__ double s_w[kNormThreads / 32];
   NormAcc acc{0.0, 0u};
-  int at = 0;
+  int at = entry_of(list, blockIdx.x);
   for (uint32_t unit = blockIdx.x; unit < list.units; unit += gridDim.x) {
     while (at + 1 < list.n && list.unit0[at + 1] <= unit) ++at;
     const GradEntry& e = list.e[at];
@@ -229,6 +252,7 @@ __device__ __forceinline__ float norm_of(int norm_type, const double* partial, i
     for (int w = 0; w < kNormThreads / 32; ++w) v = fmax(v, s_w[w]);
     return __uint_as_float((uint32_t)v);  // the bits of |x|: whole numbers below 2^32
   }
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += kNormThreads) v += partial[i];
   v = block_sum(v, s_w);
   return (float)(norm_type == kNormL2 ? sqrt(v) : v);
@@ -300,7 +324,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocksPerSm) clip_kernel(co
   }
   const double ratio = c.max_norm / ((double)norm + 1e-6);
   const float coef = ratio >= 1.0 ? 1.f : (float)ratio;  // a NaN ratio stays
-  int at = list.n - 1;
+  int at = entry_of(list, list.units - 1 - blockIdx.x);
   for (uint32_t i = blockIdx.x; i < list.units; i += gridDim.x) {
     const uint32_t unit = list.units - 1 - i;
     while (list.unit0[at] > unit) --at;

@@ -271,78 +271,88 @@ static bool fill_list(GradList<SLOTS>& list, const moe_tensor_desc* t, int n, in
   return list.n > 0;
 }
 
-static int norm_blocks(uint32_t units, int sms) {
-  return (int)std::min<int64_t>(units, std::min(kNormMaxBlocks, sms * kNormBlocksPerSm));
+static bool norm_large(const moe_tensor_desc* t, int n) {
+  uint64_t units = 0;
+  for (int i = 0; i < n; ++i) units += ((uint64_t)t[i].rows * t[i].cols) / unit_elems(t[i].in_type) + 1;
+  return units > kNormLarge;
 }
 
 template <int NORM, int SLOTS>
-static int launch_partials(const moe_tensor_desc* t, int n, double* partial, int* count, int sms, cudaStream_t st) {
+static int launch_partials(const moe_tensor_desc* t, int n, bool large, double* partial, int* count, cudaStream_t st) {
   int at = 0;
   *count = 0;
   GradList<SLOTS> list;
   while (fill_list(list, t, n, &at, -1)) {
-    const int blocks = norm_blocks(list.units, sms);
+    const int blocks = (int)std::min<uint32_t>(list.units, large ? kNormMaxBlocks : kNormResident);
     norm_partial_kernel<NORM, SLOTS><<<blocks, kNormThreads, 0, st>>>(list, partial + *count);
     MOE_CUDA_TRY(cudaGetLastError());
     *count += blocks;
   }
   return 0;
 }
+template <int NORM>
+static int run_partials(const moe_tensor_desc* t, int n, bool large, double* partial, int* count, cudaStream_t st) {
+  if (n <= kGradSlotsSmall) return launch_partials<NORM, kGradSlotsSmall>(t, n, large, partial, count, st);
+  return launch_partials<NORM, kGradSlots>(t, n, large, partial, count, st);
+}
+// The partials of all tensors; their number.
+static int norm_partials(int norm_type, const moe_tensor_desc* t, int n, bool large, double* partial, int* count,
+                         cudaStream_t st) {
+  if (norm_type == MOE_NORM_L1) return run_partials<kNormL1>(t, n, large, partial, count, st);
+  if (norm_type == MOE_NORM_L2) return run_partials<kNormL2>(t, n, large, partial, count, st);
+  return run_partials<kNormInf>(t, n, large, partial, count, st);
+}
+
 template <int SLOTS, int IN, int OUT>
-static int launch_clip_pair(const moe_tensor_desc* t, int n, ClipNorm* c, int sms, cudaStream_t st) {
+static int launch_clip_pair(const moe_tensor_desc* t, int n, bool large, ClipNorm* c, cudaStream_t st) {
   int at = 0;
   GradList<SLOTS> list;
   while (fill_list(list, t, n, &at, IN * 3 + OUT)) {
-    clip_kernel<IN, OUT, SLOTS><<<norm_blocks(list.units, sms), kNormThreads, 0, st>>>(list, *c);
+    const uint32_t blocks = large ? list.units : std::min<uint32_t>(list.units, kNormResident);
+    clip_kernel<IN, OUT, SLOTS><<<blocks, kNormThreads, 0, st>>>(list, *c);
     MOE_CUDA_TRY(cudaGetLastError());
     c->norm = nullptr;  // the first launch writes it
   }
   return 0;
 }
 template <int SLOTS>
-static int launch_clip(const moe_tensor_desc* t, int n, ClipNorm c, int sms, cudaStream_t st) {
+static int launch_clip(const moe_tensor_desc* t, int n, bool large, ClipNorm c, cudaStream_t st) {
   unsigned pairs = 0;
   for (int i = 0; i < n; ++i)
     if (t[i].rows && t[i].cols) pairs |= 1u << type_pair(t[i]);
   int r = 0;
-  if (!r && (pairs & 1u)) r = launch_clip_pair<SLOTS, 0, 0>(t, n, &c, sms, st);
-  if (!r && (pairs & 2u)) r = launch_clip_pair<SLOTS, 0, 1>(t, n, &c, sms, st);
-  if (!r && (pairs & 4u)) r = launch_clip_pair<SLOTS, 0, 2>(t, n, &c, sms, st);
-  if (!r && (pairs & 8u)) r = launch_clip_pair<SLOTS, 1, 0>(t, n, &c, sms, st);
-  if (!r && (pairs & 16u)) r = launch_clip_pair<SLOTS, 1, 1>(t, n, &c, sms, st);
-  if (!r && (pairs & 32u)) r = launch_clip_pair<SLOTS, 1, 2>(t, n, &c, sms, st);
-  if (!r && (pairs & 64u)) r = launch_clip_pair<SLOTS, 2, 0>(t, n, &c, sms, st);
-  if (!r && (pairs & 128u)) r = launch_clip_pair<SLOTS, 2, 1>(t, n, &c, sms, st);
-  if (!r && (pairs & 256u)) r = launch_clip_pair<SLOTS, 2, 2>(t, n, &c, sms, st);
+  if (!r && (pairs & 1u)) r = launch_clip_pair<SLOTS, 0, 0>(t, n, large, &c, st);
+  if (!r && (pairs & 2u)) r = launch_clip_pair<SLOTS, 0, 1>(t, n, large, &c, st);
+  if (!r && (pairs & 4u)) r = launch_clip_pair<SLOTS, 0, 2>(t, n, large, &c, st);
+  if (!r && (pairs & 8u)) r = launch_clip_pair<SLOTS, 1, 0>(t, n, large, &c, st);
+  if (!r && (pairs & 16u)) r = launch_clip_pair<SLOTS, 1, 1>(t, n, large, &c, st);
+  if (!r && (pairs & 32u)) r = launch_clip_pair<SLOTS, 1, 2>(t, n, large, &c, st);
+  if (!r && (pairs & 64u)) r = launch_clip_pair<SLOTS, 2, 0>(t, n, large, &c, st);
+  if (!r && (pairs & 128u)) r = launch_clip_pair<SLOTS, 2, 1>(t, n, large, &c, st);
+  if (!r && (pairs & 256u)) r = launch_clip_pair<SLOTS, 2, 2>(t, n, large, &c, st);
   return r;
 }
-template <int NORM>
-static int run_norm(const moe_tensor_desc* t, int n, float* norm, double* partial, int sms, cudaStream_t st) {
-  int count = 0;
-  const int r = n <= kGradSlotsSmall ? launch_partials<NORM, kGradSlotsSmall>(t, n, partial, &count, sms, st)
-                                     : launch_partials<NORM, kGradSlots>(t, n, partial, &count, sms, st);
-  if (r) return r;
-  norm_finish_kernel<<<1, kNormThreads, 0, st>>>(NORM, partial, count, norm);
-  MOE_CUDA_TRY(cudaGetLastError());
-  return 0;
-}
-template <int NORM>
-static int run_clip(const moe_tensor_desc* t, int n, double max_norm, const float* given, float* norm, double* partial,
-                    int sms, cudaStream_t st) {
-  ClipNorm c{partial, 0, NORM, given, norm, max_norm};
-  const bool small = n <= kGradSlotsSmall;
+
+static int run_clip(const moe_tensor_desc* t, int n, int norm_type, double max_norm, const float* given, float* norm,
+                    double* partial, cudaStream_t st) {
+  const bool large = norm_large(t, n);
+  ClipNorm c{partial, 0, norm_type, given, norm, max_norm};
   if (!given) {
-    const int r = small ? launch_partials<NORM, kGradSlotsSmall>(t, n, partial, &c.n, sms, st)
-                        : launch_partials<NORM, kGradSlots>(t, n, partial, &c.n, sms, st);
-    if (r) return r;
+    if (int r = norm_partials(norm_type, t, n, large, partial, &c.n, st)) return r;
     if (c.n == 0) {  // no elements: the norm is 0 and there is nothing to scale
       MOE_CUDA_TRY(cudaMemsetAsync(norm, 0, sizeof(float), st));
       return 0;
     }
+    if (large) {
+      norm_finish_kernel<<<1, kNormThreads, 0, st>>>(norm_type, partial, c.n, norm);
+      MOE_CUDA_TRY(cudaGetLastError());
+      c.given = norm;
+    }
   } else if (norm && norm != given) {
     MOE_CUDA_TRY(cudaMemcpyAsync(norm, given, sizeof(float), cudaMemcpyDeviceToDevice, st));
   }
-  return small ? launch_clip<kGradSlotsSmall>(t, n, c, sms, st) : launch_clip<kGradSlots>(t, n, c, sms, st);
+  return n <= kGradSlotsSmall ? launch_clip<kGradSlotsSmall>(t, n, large, c, st)
+                              : launch_clip<kGradSlots>(t, n, large, c, st);
 }
 
 }  // namespace moe
@@ -545,9 +555,11 @@ int moe_grad_norm(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type, 
   if (int r = device_info(&dev, &di)) return r;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
-  if (norm_type == MOE_NORM_L1) return run_norm<kNormL1>(tensors, n, norm, partial, di->sms, st);
-  if (norm_type == MOE_NORM_L2) return run_norm<kNormL2>(tensors, n, norm, partial, di->sms, st);
-  return run_norm<kNormInf>(tensors, n, norm, partial, di->sms, st);
+  int count = 0;
+  if (int r = norm_partials(norm_type, tensors, n, norm_large(tensors, n), partial, &count, st)) return r;
+  norm_finish_kernel<<<1, kNormThreads, 0, st>>>(norm_type, partial, count, norm);
+  MOE_CUDA_TRY(cudaGetLastError());
+  return 0;
 }
 
 int moe_clip_grads(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type, double max_norm,
@@ -562,11 +574,8 @@ int moe_clip_grads(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type,
   int dev;
   DevInfo* di;
   if (int r = device_info(&dev, &di)) return r;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  double* partial = static_cast<double*>(workspace);
-  if (norm_type == MOE_NORM_L1) return run_clip<kNormL1>(tensors, n, max_norm, given_norm, norm, partial, di->sms, st);
-  if (norm_type == MOE_NORM_L2) return run_clip<kNormL2>(tensors, n, max_norm, given_norm, norm, partial, di->sms, st);
-  return run_clip<kNormInf>(tensors, n, max_norm, given_norm, norm, partial, di->sms, st);
+  return run_clip(tensors, n, norm_type, max_norm, given_norm, norm, static_cast<double*>(workspace),
+                  static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
