@@ -61,7 +61,7 @@ static int64_t route_counters(int64_t chunks, int64_t sequences, int E) {
 
 template <int G, int V, int KMAX>
 static int launch_route(const RouteParams& p, int64_t blocks, cudaStream_t st) {
-  const size_t smem = (size_t)p.E * sizeof(int) + (size_t)kRouteWarps * G * V * sizeof(float);
+  const size_t smem = (size_t)kRouteWarps * 32 * V * sizeof(float) + (size_t)p.E * sizeof(int);
   route_train_kernel<G, V, KMAX><<<(unsigned)blocks, kRouteThreads, smem, st>>>(p);
   MOE_CUDA_TRY(cudaGetLastError());
   return 0;

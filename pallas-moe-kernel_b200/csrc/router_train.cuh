@@ -499,7 +499,10 @@ template <int G, int V, int KMAX>
 __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_train_kernel(const RouteParams p) {
   constexpr int TPW = 32 / G;                // tokens per warp and step
   constexpr int KS = (KMAX + G - 1) / G;     // slots per lane
-  extern __shared__ int s_cnt[];             // [E] counts, then [warps][G V] sums of q
+  // [warps][V / 4][32] fours of the rows in work; after them [warps][G V] sums
+  // of q; then [E] counts.
+  extern __shared__ float4 s_quads[];
+  int* s_cnt = reinterpret_cast<int*>(s_quads + kRouteWarps * 8 * V);
   __shared__ double s_w[3 * kRouteWarps];
   __shared__ double s_fq[kRouteThreads];
   __shared__ int s_fc[kRouteThreads];
@@ -565,14 +568,20 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) acc.p[i] = __ffma2_rn(ex.p[i], both(inv), acc.p[i]);
 
-    // Choice: k rounds of the row's maximum.
+    // Choice: k rounds of the row's maximum.  A lane's logits lie in shared
+    // memory in fours with the maxima of the fours in registers: taking one
+    // out costs a search of the maxima and of one four (searching V registers
+    // took twice the instructions).  NaN equals no maximum.
     if (!p.given) {
+      constexpr int Q = V / 4;
+      float4* quads = s_quads + warp * 32 * Q + lane;
+      float qm[Q];
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) {  // NaN is never chosen
-        v.p[i].x = v.p[i].x > -INFINITY ? v.p[i].x : -INFINITY;
-        v.p[i].y = v.p[i].y > -INFINITY ? v.p[i].y : -INFINITY;
+      for (int q = 0; q < Q; ++q) {
+        const float4 x = make_float4(v.p[2 * q].x, v.p[2 * q].y, v.p[2 * q + 1].x, v.p[2 * q + 1].y);
+        quads[q * 32] = x;
+        qm[q] = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
       }
-      m = lane_max(v);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         id[s] = -1;
@@ -586,18 +595,26 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
         const int owner = __ffs(owners) - 1;
         int at = -1;
         if (lane == owner) {
+          int q = 0;
 #pragma unroll
-          for (int i = V / 2 - 1; i >= 0; --i) {
-            if (v.p[i].y == M) at = 2 * i + 1;
-            if (v.p[i].x == M) at = 2 * i;
-          }
+          for (int i = Q - 1; i > 0; --i)
+            if (qm[i] == M) q = i;
+          if (qm[0] == M) q = 0;
+          float4 x = quads[q * 32];
+          const int i = x.x == M ? 0 : x.y == M ? 1 : x.z == M ? 2 : 3;
+          if (i == 0) x.x = -INFINITY;
+          if (i == 1) x.y = -INFINITY;
+          if (i == 2) x.z = -INFINITY;
+          if (i == 3) x.w = -INFINITY;
+          quads[q * 32] = x;
+          const float left = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+          m = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < V / 2; ++i) {
-            if (2 * i == at) v.p[i].x = -INFINITY;
-            if (2 * i + 1 == at) v.p[i].y = -INFINITY;
+          for (int z = 0; z < Q; ++z) {
+            if (z == q) qm[z] = left;
+            m = fmaxf(m, qm[z]);
           }
-          m = lane_max(v);
-          at += e0;
+          at = e0 + 4 * q + i;
         }
         at = __shfl_sync(0xffffffffu, at, owner < 0 ? lane : owner);
         if (gl == j % G) {
@@ -651,7 +668,8 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     z += __shfl_xor_sync(0xffffffffu, z, o);
     n += __shfl_xor_sync(0xffffffffu, n, o);
   }
-  float* s_q = reinterpret_cast<float*>(s_cnt + E);
+  float* s_q = reinterpret_cast<float*>(s_quads);
+  __syncthreads();
   if (lane < G) {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
