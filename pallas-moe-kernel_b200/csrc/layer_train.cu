@@ -213,6 +213,9 @@ static int check_outputs(const moe_tensor_desc* t, int n) {
   auto live = [&](int i) { return t[i].rows && t[i].cols; };
   int last = -1;
   bool sorted = true, apart = true;
+  for (int i = 0; i < n; ++i)
+    if (live(i) && t[i].out == t[i].in && (t[i].in_type != t[i].out_type || (t[i].rows > 1 && t[i].in_ld != t[i].out_ld)))
+      return fail(MOE_ERR_INVALID_ARG, "tensor %d is scaled in place with another type or stride", i);
   for (int i = 0; i < n; ++i) {
     if (!live(i)) continue;
     if (last >= 0 && start(i) < end(last)) {

@@ -105,6 +105,7 @@ class RouteTrain(NamedTuple):
 
 _ELEMS = {torch.float32: _lib.MOE_ELEM_F32, torch.bfloat16: _lib.MOE_ELEM_BF16, torch.float16: _lib.MOE_ELEM_F16}
 _SCORING = {"softmax": 0, "sigmoid": 1}
+_ROUTED_TYPES = (torch.int32, torch.float32, torch.int32, torch.int32)  # ids, weights, counts, tokens
 
 
 def _elem(t: torch.Tensor, name: str) -> int:
@@ -232,6 +233,8 @@ def route_forward_train(logits: torch.Tensor, k: int, *, ids: Optional[torch.Ten
         _on(dev, ids=ids)
         if ids.dtype.is_floating_point or ids.dtype == torch.bool:
             raise TypeError(f"ids are {ids.dtype}, not integers")
+        if ids.dtype == torch.int64:
+            ids = ids.clamp(-1, E)             # far values stay out of range in 32 bits
         ids = ids.to(torch.int32).contiguous()
     if not 1 <= k <= min(16, E) or E > 1024:
         raise ValueError(f"k={k}, E={E}: 1 <= k <= min(16, E) and E <= 1024 are supported")
@@ -257,11 +260,15 @@ def route_backward(logits: torch.Tensor, routed: RouteTrain, *, d_weights: Optio
     logits, code, ld, mask_ptr, how, mask = _route_args(logits, mask, sequences, scoring)
     dev = logits.device
     T, E = logits.shape
-    ids, weights, counts, tokens = routed[:4]
+    ids, weights, counts, tokens = saved = routed[:4]
     k = ids.shape[-1]
-    if ids.shape != (T, k) or counts.shape != (sequences, E) or ids.device != dev:
-        raise ValueError(f"routed has ids {tuple(ids.shape)} and counts {tuple(counts.shape)} on {ids.device}, "
-                         f"expected {(T, k)} and {(sequences, E)} on {dev}")
+    if (ids.shape != (T, k) or weights.shape != (T, k) or counts.shape != (sequences, E) or tokens.shape != (sequences,)
+            or ids.device != dev):
+        raise ValueError(f"routed has ids {tuple(ids.shape)}, weights {tuple(weights.shape)}, counts "
+                         f"{tuple(counts.shape)} and tokens {tuple(tokens.shape)} on {ids.device}, expected {(T, k)}, "
+                         f"{(T, k)}, {(sequences, E)} and {(sequences,)} on {dev}")
+    if tuple(t.dtype for t in saved) != _ROUTED_TYPES or not all(map(torch.Tensor.is_contiguous, saved)):
+        raise TypeError("routed's tensors must be as route_forward_train returns them: int32 and float32, contiguous")
     if d_weights is not None:
         if d_weights.shape != (T, k) or d_weights.device != dev:
             raise ValueError(f"d_weights is {tuple(d_weights.shape)} on {d_weights.device}, expected {(T, k)} on {dev}")

@@ -21,6 +21,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import router
@@ -251,6 +252,7 @@ class RouteTopK(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, _ids, dw, _counts, _tokens, d_balance, d_z):
         logits, mask, ids, weights, counts, tokens = ctx.saved_tensors
         if dw is None and d_balance is None and d_z is None:
@@ -284,11 +286,12 @@ class RoutedExperts(torch.autograd.Function):
         return router.combine_rows(ys, inv, weights)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         xs, weights, w_in, w_down, gs, inv, ys, saved = ctx.saved_tensors
         dys, dw = router.combine_rows_backward(dy, ys, inv, weights, gs, dtype=torch.bfloat16)
         dxs, dw_in, dw_down = (swiglu_backward if ctx.swiglu else backward)(xs, w_in, w_down, gs, saved, dys)
-        dx = router.gather_rows_backward(dxs, inv, dtype=xs.dtype)
+        dx = router.gather_rows_backward(dxs, inv, dtype=xs.dtype) if ctx.needs_input_grad[0] else None
         return dx, dw, dw_in.to(w_in.dtype), dw_down.to(w_down.dtype), None, None
 
 
@@ -311,6 +314,8 @@ def moe_layer_train(x: torch.Tensor, logits: torch.Tensor, w_in: torch.Tensor, w
     if activation not in ("gelu", "swiglu"):
         raise ValueError(f"activation {activation!r} is not 'gelu' or 'swiglu'")
     M, D, F, E = (_check_swiglu if activation == "swiglu" else _check)(x, w_in, w_down)
+    if M == 0:
+        raise ValueError("moe_layer_train needs at least one token")
     if tuple(logits.shape) != (M, E) or logits.device != x.device:
         raise ValueError(f"logits {tuple(logits.shape)} on {logits.device}: expected {(M, E)} on {x.device}")
     with torch.cuda.device(x.device):

@@ -197,6 +197,7 @@ def test_gradient_list_abi_refusals():
         return L.moe_clip_grads(d, 2, 2, 1.0, None, p, p, 8, None)
     assert pair(256, 256, 1, 1) == pair(256, 260, 2, 1) == pair(260, 256, 1, 2) == -1
     assert b"share memory" in L.moe_last_error()
+    assert clip(out_type=1) == clip(rows=2, out_ld=12) == -1       # in place, but not the same elements
     assert pair(256, 260, 1, 1) == pair(260, 256, 1, 1) == pair(256, 256, 0, 1) == -4      # apart: the workspace is next
     assert L.moe_grad_norm_workspace_size(-1) == 0 and L.moe_grad_norm_workspace_size(1000) > L.moe_grad_norm_workspace_size(1)
 

@@ -273,6 +273,27 @@ def test_route_python_refusals():
         router.route_backward(x, r, d_balance=torch.zeros(2, device=DEV))
     with pytest.raises(ValueError, match="routed"):
         router.route_backward(x[:3], r)
+    with pytest.raises(TypeError, match="routed"):
+        router.route_backward(x, r._replace(weights=r.weights.half()))
+    with pytest.raises(TypeError, match="ids"):
+        router.route_forward_train(x, 2, ids=torch.zeros((4, 2), device=DEV))
+
+
+def test_route_offsets_past_32_bits_and_wide_ids():
+    """Rows four billion elements from the first, and ids that 32 bits would wrap."""
+    base = torch.zeros((4400, 1_000_000), dtype=torch.bfloat16, device=DEV)
+    x, dw = _logits(4400, 64, torch.bfloat16, 13)
+    base[:, :64] = x
+    want = router.route_forward_train(x, 6)
+    got = router.route_forward_train(base[:, :64], 6)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(router.route_backward(base[:, :64], got, d_weights=dw[:, :6]),
+                       router.route_backward(x, want, d_weights=dw[:, :6]))
+    ids = want.ids.long()
+    ids[0, 0], ids[1, 1] = 2 ** 32 + 3, -(2 ** 32) + 5
+    far = router.route_forward_train(x, 6, ids=ids)
+    assert far.ids[0, 0].item() == -1 and far.ids[1, 1].item() == -1
 
 
 # ----------------------------------------------------------------------------- rows
@@ -366,6 +387,25 @@ def test_rows_strides_bad_indexes_and_refusals():
         router.combine_rows_backward(dy, ys, inv, w[:3], gs)
     with pytest.raises(TypeError):
         router.gather_rows_backward(ys, inv, dtype=torch.float64)
+
+
+def test_rows_past_32_bits():
+    T, k, D = 270_000, 2, 8192                                     # 4.4 billion elements of expert rows
+    inv = torch.arange(T * k - 1, -1, -1, dtype=torch.int32, device=DEV).view(T, k)
+    dxs = torch.zeros((T * k, D), dtype=torch.bfloat16, device=DEV)
+    dxs[0], dxs[-1], dxs[-2] = 1.0, 2.0, 3.0
+    dx = router.gather_rows_backward(dxs, inv)
+    assert torch.all(dx[0] == 5.0) and torch.all(dx[-1] == 1.0) and dx[1:-1].abs().max().item() == 0
+    del dxs, dx
+    ys = torch.zeros((T * k, D), device=DEV)
+    ys[-1], ys[0] = 2.0, 1.0
+    dy = torch.zeros((T, D), dtype=torch.bfloat16, device=DEV)
+    dy[0], dy[-1] = 1.0, 0.5
+    w = torch.full((T, k), 0.25, device=DEV)
+    gs = torch.tensor([T * k], dtype=torch.int32, device=DEV)
+    dys, dw = router.combine_rows_backward(dy, ys, inv, w, gs, dtype=torch.bfloat16)
+    assert dw[0].tolist() == [2.0 * D, 0.0] and dw[-1].tolist() == [0.0, 0.5 * D]
+    assert torch.all(dys[-2:] == 0.25) and torch.all(dys[:2] == 0.125) and dys[2:-2].abs().max().item() == 0
 
 
 # ----------------------------------------------------------------------------- gradient norm and clipping
@@ -464,6 +504,36 @@ def test_clip_strides_offsets_and_given_norm():
     t = torch.ones(100, device=DEV)
     assert grads.clip_grads([t], 1.0, total) is total
     _close(t, np.full(100, 1 / (4 + 1e-6)), 3 * U * 0.25)
+
+
+def test_clip_past_32_bits():
+    """More elements than 32 bits count: dense, and rows that are a slice."""
+    t = torch.zeros(2 ** 32 + 1003, dtype=torch.bfloat16, device=DEV)
+    t[0], t[2 ** 32 + 5], t[-1] = 3.0, 4.0, 12.0
+    assert grads.clip_grad_norm([t], 6.5).item() == 13.0
+    # 6.5 / (13 + 1e-6) is 0.5 less 4e-8 of it: each product rounds to half of its element.
+    assert t[0].item() == 1.5 and t[2 ** 32 + 5].item() == 2.0 and t[-1].item() == 6.0
+    rows = t[:2 ** 32].view(2, 2 ** 31)[:, :2 ** 31 - 8]
+    rows[0, -1], rows[1, -1] = 4.0, -6.0
+    rows[0, 0] = 12.0
+    assert grads.clip_grad_norm([rows], 7.0).item() == 14.0
+    assert rows[0, -1].item() == 2.0 and rows[1, -1].item() == -3.0 and rows[0, 0].item() == 6.0
+
+
+def test_clip_large_lists_take_the_other_path():
+    """Above 155 MB the norm has a launch of its own and every block takes one unit."""
+    ts = _tensors([30_000_001, 17, 12_345_678], torch.float32, 5)
+    want = float(torch.cat(ts).double().square().sum().sqrt())
+    out = [torch.empty_like(t, dtype=torch.bfloat16) for t in ts]
+    norm = grads.clip_grad_norm(ts, 0.3 * want, out=out)
+    assert abs(norm.item() - want) <= _norm_tol(2) * want
+    for o, t in zip(out, ts):
+        ref = t.double() * (0.3 * want / (want + 1e-6))
+        assert torch.all((o.double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 20 * U))
+    again = [torch.empty_like(o) for o in out]
+    assert torch.equal(norm, grads.clip_grad_norm(ts, 0.3 * want, out=again))
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+    assert grads.grad_norm(ts, math.inf).item() == max(t.abs().max().item() for t in ts)
 
 
 def test_clip_repeats_on_streams_and_in_a_graph():
@@ -644,3 +714,48 @@ def test_layer_step_in_a_graph():
             assert torch.equal(a, b)
     del graph
     assert _lib.device_status(reset=True) == 0
+
+
+def test_layer_backward_in_a_graph():
+    """An autograd step captured whole, on leaves without an eager graph, and replayed."""
+    T, D, F, E, k = 128, 256, 256, 4, 2
+    x0, wr, ups, wd, dy = _layer_inputs(T, D, F, E, False, 11)
+
+    def leaves(x):
+        return [t.detach().clone().requires_grad_() for t in (x, wr, ups[0], wd)]
+
+    def step(x, wr, wu, wd):
+        y, routed = train.moe_layer_train(x, x.float() @ wr, wu, wd, k)
+        loss = (y * dy).sum() + 0.01 * routed.balance_loss
+        return torch.autograd.grad(loss, (x, wr, wu, wd))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(*leaves(x0))                                          # warm-up; its graph is gone at the return
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    static = leaves(x0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for seed in (1, 2):
+        new = _layer_inputs(T, D, F, E, False, seed)[0]
+        with torch.no_grad():
+            static[0].copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(*leaves(new))):
+            assert torch.equal(a, b)
+    del graph
+
+
+def test_layer_second_derivatives_are_refused():
+    T, D, F, E, k = 64, 256, 256, 4, 2
+    x, wr, ups, wd, dy = _layer_inputs(T, D, F, E, False, 12)
+    logits = (x.float() @ wr).requires_grad_()
+    r = train.route_topk_train(logits, k)
+    d, = torch.autograd.grad(r.balance_loss, logits, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+    with pytest.raises(ValueError, match="token"):
+        train.moe_layer_train(x[:0], logits[:0], ups[0], wd, k)
