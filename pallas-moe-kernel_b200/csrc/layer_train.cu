@@ -26,13 +26,12 @@ static int route_lanes(int E) {
 }
 
 // Blocks per sequence: enough that a warp has one step of tokens, and at most
-// kRouteBlocks over all sequences where a sequence is longer than that (what
-// is resident at 80 registers a thread: a second, short wave costs its whole
-// length).
-constexpr int64_t kRouteBlocks = 148 * 3;
+// as many over all sequences as are resident (3 an SM at 80 registers a thread,
+// 2 at 128): a second, short wave costs its whole length.
+static int64_t route_blocks(int E) { return 148 * (E > 512 ? 2 : 3); }
 static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
   const int64_t step = kRouteWarps * (32 / route_lanes(E));
-  const int64_t most = std::max<int64_t>(1, kRouteBlocks / std::max<int64_t>(1, sequences));
+  const int64_t most = std::max<int64_t>(1, route_blocks(E) / std::max<int64_t>(1, sequences));
   return std::max<int64_t>(1, std::min((seq_len + step - 1) / step, most));
 }
 
@@ -103,9 +102,14 @@ static int check_route(int elem_type, int64_t ld, int64_t T, int E, int k, int64
   return 0;
 }
 
-// Rows of whole 16-byte vectors, eight elements at a time.
-static bool route_vec(const void* base, int64_t ld, int E, int type) {
-  return E % 8 == 0 && aligned16(base) && (size_t)ld * elem_bytes(type) % 16 == 0;
+// Elements of a row that can be read or written at a time: 8, 4 or 1.
+static int route_vec(const void* base, int64_t ld, int E, int type) {
+  for (int v = 8; v > 1; v /= 2) {
+    const size_t bytes = std::min<size_t>(16, v * elem_bytes(type));
+    if (E % v == 0 && ld % v == 0 && reinterpret_cast<uintptr_t>(base) % bytes == 0) return v;
+    if (v == 4) break;
+  }
+  return 1;
 }
 
 // ------------------------------------------------------------------ rows
