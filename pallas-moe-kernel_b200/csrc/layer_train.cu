@@ -71,20 +71,21 @@ static int launch_route_k(const RouteParams& p, int64_t blocks, cudaStream_t st)
   if (p.k <= 8) return launch_route<G, V, 8>(p, blocks, st);
   return launch_route<G, V, 16>(p, blocks, st);
 }
-template <int G, int V, int KMAX>
+template <int G, int V, int KMAX, bool WEIGHTS>
 static int launch_backward(const RouteBackward& p, int64_t blocks, cudaStream_t st) {
-  route_backward_kernel<G, V, KMAX><<<(unsigned)blocks, kRouteThreads, 0, st>>>(p);
+  route_backward_kernel<G, V, KMAX, WEIGHTS><<<(unsigned)blocks, kRouteThreads, 0, st>>>(p);
   MOE_CUDA_TRY(cudaGetLastError());
   return 0;
 }
 template <int G, int V>
 static int launch_backward_k(const RouteBackward& p, int64_t blocks, cudaStream_t st) {
+  if (!p.d_weights) return launch_backward<G, V, G, false>(p, blocks, st);
   if constexpr (G >= kRouteMaxK) {
-    return launch_backward<G, V, kRouteMaxK>(p, blocks, st);  // one slot a lane
+    return launch_backward<G, V, kRouteMaxK, true>(p, blocks, st);  // one slot a lane
   } else {
-    if (p.k <= 2) return launch_backward<G, V, 2>(p, blocks, st);
-    if (p.k <= 8) return launch_backward<G, V, 8>(p, blocks, st);
-    return launch_backward<G, V, kRouteMaxK>(p, blocks, st);
+    if (p.k <= 2) return launch_backward<G, V, 2, true>(p, blocks, st);
+    if (p.k <= 8) return launch_backward<G, V, 8, true>(p, blocks, st);
+    return launch_backward<G, V, kRouteMaxK, true>(p, blocks, st);
   }
 }
 

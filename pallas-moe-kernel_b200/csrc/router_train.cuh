@@ -160,40 +160,59 @@ __device__ __forceinline__ void row_load(const void* p, int type, int vec, int64
   else if (type == kElemBF16) row_load_t<kElemBF16>(p, vec, row, e0, E, live, v);
   else row_load_t<kElemF16>(p, vec, row, e0, E, live, v);
 }
-template <int TYPE, int V>
-__device__ __forceinline__ void row_put_t(void* p, int vec, int64_t row, int e0, int E, const Row<V>& v) {
+// A warp's rows in shared memory, 32 V floats in fours: four q of lane l lies
+// at q * 32 + (l ^ q * 32 / V), which neither the lanes' own fours (one q, all
+// lanes) nor fours in the order of the experts (all q of a lane, next lane)
+// find in one bank.
+template <int V>
+__device__ __forceinline__ int four_at(int l, int q) {
+  return q * 32 + (l ^ (q * (32 / V)));
+}
+
+// Stores the warp's 32 / G rows from shared memory, neighbouring lanes
+// neighbouring experts: a lane's own V experts written in 16-byte pieces are
+// half sectors, twice as many requests.
+template <int TYPE, int G, int V>
+__device__ __forceinline__ void rows_store_t(const float4* s_fours, void* p, int vec, int64_t t0, int64_t hi, int E,
+                                             int lane) {
   if (vec == 8 && TYPE != kElemF32) {
 #pragma unroll
-    for (int c = 0; c < V; c += 8) {
-      const float2* q = v.p + c / 2;
-      if (e0 + c < E)
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + e0 + c) =
-            make_uint4(pack16(q[0].x, q[0].y, TYPE), pack16(q[1].x, q[1].y, TYPE), pack16(q[2].x, q[2].y, TYPE),
-                       pack16(q[3].x, q[3].y, TYPE));
+    for (int i = 0; i < V / 8; ++i) {
+      const int at = i * 32 + lane, l = at / (V / 8), e = 8 * (at % (G * V / 8));
+      const int64_t t = t0 + l / G;
+      if (t >= hi || e >= E) continue;
+      const float4 x = s_fours[four_at<V>(l, 2 * (at % (V / 8)))], y = s_fours[four_at<V>(l, 2 * (at % (V / 8)) + 1)];
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + t * E + e) =
+          make_uint4(pack16(x.x, x.y, TYPE), pack16(x.z, x.w, TYPE), pack16(y.x, y.y, TYPE), pack16(y.z, y.w, TYPE));
     }
   } else if (vec >= 4) {
 #pragma unroll
-    for (int c = 0; c < V; c += 4) {
-      const float2* q = v.p + c / 2;
-      if (e0 + c >= E) continue;
+    for (int i = 0; i < V / 4; ++i) {
+      const int at = i * 32 + lane, l = at / (V / 4), e = 4 * (at % (G * V / 4));
+      const int64_t t = t0 + l / G;
+      if (t >= hi || e >= E) continue;
+      const float4 x = s_fours[four_at<V>(l, at % (V / 4))];
       if (TYPE == kElemF32)
-        *reinterpret_cast<float4*>(static_cast<float*>(p) + row + e0 + c) =
-            make_float4(q[0].x, q[0].y, q[1].x, q[1].y);
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + t * E + e) = x;
       else
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + row + e0 + c) =
-            make_uint2(pack16(q[0].x, q[0].y, TYPE), pack16(q[1].x, q[1].y, TYPE));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + t * E + e) =
+            make_uint2(pack16(x.x, x.y, TYPE), pack16(x.z, x.w, TYPE));
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (e0 + i < E) elem_store(p, TYPE, row + e0 + i, i & 1 ? v.p[i / 2].y : v.p[i / 2].x);
+    for (int i = 0; i < V; ++i) {
+      const int at = i * 32 + lane, l = at / V, e = at % (G * V);
+      const int64_t t = t0 + l / G;
+      if (t < hi && e < E)
+        elem_store(p, TYPE, t * E + e, reinterpret_cast<const float*>(s_fours + four_at<V>(l, at % V / 4))[at % 4]);
+    }
   }
 }
-template <int V>
-__device__ __forceinline__ void row_put(void* p, int type, int vec, int64_t row, int e0, int E, const Row<V>& v) {
-  if (type == kElemF32) row_put_t<kElemF32>(p, vec, row, e0, E, v);
-  else if (type == kElemBF16) row_put_t<kElemBF16>(p, vec, row, e0, E, v);
-  else row_put_t<kElemF16>(p, vec, row, e0, E, v);
+template <int G, int V>
+__device__ __forceinline__ void rows_store(const float4* s_fours, void* p, int type, int vec, int64_t t0, int64_t hi,
+                                           int E, int lane) {
+  if (type == kElemF32) rows_store_t<kElemF32, G, V>(s_fours, p, vec, t0, hi, E, lane);
+  else if (type == kElemBF16) rows_store_t<kElemBF16, G, V>(s_fours, p, vec, t0, hi, E, lane);
+  else rows_store_t<kElemF16, G, V>(s_fours, p, vec, t0, hi, E, lane);
 }
 template <int V>
 __device__ __forceinline__ void row_fill(Row<V>& v, float x) {
@@ -503,16 +522,14 @@ __device__ __forceinline__ void route_finish(const RouteParams& p, int64_t seq, 
   }
 }
 
-// Blocks per SM that the register budget is cut for.  E = 1024, T = 32768, f32:
-// the forward runs 139 us at one block of 190 registers a thread and 113 at two
-// of 128, the backward 128 and 156 (it holds more rows at a time).
+// Blocks per SM that the register budget is cut for.
 template <int G, int V, int KMAX>
-constexpr int route_residents(bool backward) {
-  return V == 32 ? (backward ? 1 : 2) : (KMAX + G - 1) / G <= 4 ? 3 : 2;
+constexpr int route_residents() {
+  return V == 32 ? 2 : (KMAX + G - 1) / G <= 4 ? 3 : 2;
 }
 
 template <int G, int V, int KMAX>
-__global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(false)) route_train_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_train_kernel(const RouteParams p) {
   constexpr int TPW = 32 / G;                // tokens per warp and step
   constexpr int KS = (KMAX + G - 1) / G;     // slots per lane
   // [warps][V / 4][32] fours of the rows in work; after them [warps][G V] sums
@@ -739,14 +756,14 @@ struct RouteBackward {
 //   normalised                   w_j (dw_j - <dw, w>) (times 1 - s_j, sigmoid)
 //   plain softmax probability    w_j dw_j, and -p_e <dw, w> on every expert
 //   plain sigmoid                w_j dw_j (1 - s_j)
-// It is formed in the slots' lanes and handed to the experts' lanes through a
-// row in shared memory that is zero between uses (a register exchange takes
-// k V compares a lane).
-template <int G, int V, int KMAX>
-__global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(true)) route_backward_kernel(const RouteBackward p) {
+// It is formed in the slots' lanes and added to the row in shared memory, on
+// its way to the store (a register exchange takes k V compares a lane).
+// WEIGHTS: there is such a part (the losses alone spare its registers).
+template <int G, int V, int KMAX, bool WEIGHTS>
+__global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_backward_kernel(const RouteBackward p) {
   constexpr int TPW = 32 / G;
   constexpr int KS = (KMAX + G - 1) / G;
-  __shared__ __align__(16) float s_row[kRouteWarps][32 * V];
+  __shared__ float4 s_rows[kRouteWarps][8 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gl = lane % G;
   const int e0 = gl * V, E = p.E, k = p.k;
@@ -754,10 +771,7 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
   const int chunk = blockIdx.x % p.chunks;
   const int64_t lo = seq * p.seq_len + p.seq_len * chunk / p.chunks;
   const int64_t hi = seq * p.seq_len + p.seq_len * (chunk + 1) / p.chunks;
-  float* row = s_row[warp] + (lane / G) * (G * V);
-#pragma unroll
-  for (int i = 0; i < V; ++i) s_row[warp][i * 32 + lane] = 0.f;
-  __syncwarp();
+  float4* fours = s_rows[warp];
 
   // Tokens in all sequences and sequences with any.
   const int ns = __ldg(p.tokens + seq);
@@ -776,15 +790,21 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
   // where k N E, which bounds c E, fits).
   const float db = p.d_balance && ns > 0 ? __ldg(p.d_balance) / ((float)live_seqs * (float)ns) : 0.f;
   const float dz = p.d_z && all > 0 ? 2.f * __ldg(p.d_z) / (float)all : 0.f;
-  Row<V> f;
+  // They lie in shared memory, a lane's experts in fours: the registers that
+  // they would take hold more rows instead.
+  __shared__ float4 s_f[V / 4][32];
   const float kn = db / (float)((int64_t)k * (ns > 0 ? ns : 1));
   const bool narrow = (int64_t)k * ns * E < (int64_t)1 << 31;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = e0 + i < E ? __ldg(p.counts + seq * E + e0 + i) : 0;
-    const float x = narrow ? (float)(c * E - k * ns) : (float)((int64_t)c * E - (int64_t)k * ns);
-    (i & 1 ? f.p[i / 2].y : f.p[i / 2].x) = e0 + i < E ? x * kn : 0.f;
+  for (int i = threadIdx.x; i < 32 * V; i += kRouteThreads) {
+    const int l = i / V, x = i % V, e = l % G * V + x;
+    const int c = e < E ? __ldg(p.counts + seq * E + e) : 0;
+    const float over = narrow ? (float)(c * E - k * ns) : (float)((int64_t)c * E - (int64_t)k * ns);
+    reinterpret_cast<float*>(&s_f[x / 4][l])[x % 4] = e < E ? over * kn : 0.f;
   }
+  __syncthreads();
+  const auto f = [&](int i) {  // pair i of the lane's experts
+    return reinterpret_cast<const float2*>(&s_f[i / 2][lane])[i % 2];
+  };
 
   for (int64_t base = lo + warp * TPW; base < hi; base += kRouteWarps * TPW) {
     const int64_t t = base + lane / G;
@@ -797,7 +817,7 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
     // The weights' part per slot.
     int id[KS];
     float g[KS], w[KS], dot = 0.f;
-    if (p.d_weights) {
+    if constexpr (WEIGHTS) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int j = s * G + gl;
@@ -813,6 +833,9 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
           w[s] = g[s] = 0.f;
         }
         dot = fmaf(w[s], g[s], dot);
+        // 1 - sigmoid of the slot's logit, into its weight: w is done with.
+        if (p.sigmoid && id[s] >= 0)
+          w[s] *= rcp_ftz(1.f + ex2_ftz(elem_load(p.logits, p.type, t * p.ld + id[s]) * kLog2e));
       }
     }
     const float mx = group_max<G>(lane_max(v));
@@ -820,36 +843,11 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
     const float mxl = keep ? mx * kLog2e : 0.f;
     Row<V> d;
     float total = row_exp(v, mxl, d);
-    if (p.d_weights) {
-      dot = group_sum<G>(dot);
-      const float off = p.normalize ? dot : 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        g[s] = w[s] * (g[s] - off);
-        if (p.sigmoid && id[s] >= 0)  // 1 - sigmoid, from the slot's own logit
-          g[s] *= rcp_ftz(1.f + ex2_ftz(elem_load(p.logits, p.type, t * p.ld + id[s]) * kLog2e));
-        // Slots of one expert (the caller's choice may repeat it) are added
-        // in slot order by the lowest of their lanes.
-        const int key = id[s] >= 0 ? lane / G * (G * V) + id[s] : -1 - lane;
-        const uint32_t peers = __match_any_sync(0xffffffffu, key);
-        bool mine = true;
-        if (__any_sync(0xffffffffu, peers != 1u << lane)) {
-          float sum = 0.f;
-          for (int l = 0; l < 32; ++l) {
-            const float x = __shfl_sync(0xffffffffu, g[s], l);
-            if (peers >> l & 1u) sum += x;
-          }
-          g[s] = sum;
-          mine = lane == __ffs(peers) - 1;
-        }
-        if (id[s] >= 0 && mine) row[id[s]] += g[s];
-        __syncwarp();
-      }
-    }
+    if (WEIGHTS) dot = group_sum<G>(dot);
     if (!p.sigmoid) {
       float2 fs = both(0.f);
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) fs = __ffma2_rn(f.p[i], d.p[i], fs);
+      for (int i = 0; i < V / 2; ++i) fs = __ffma2_rn(f(i), d.p[i], fs);
       total = group_sum<G>(total);
       const float fq = group_sum<G>(fs.x + fs.y);
       const float inv = keep ? rcp_ftz(total) : 0.f;
@@ -857,13 +855,13 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
       const float every = dz * ((mxl + lg2_ftz(total)) * kLn2) - fq * inv - (p.normalize ? 0.f : dot);
       const float2 x = both(inv), y = both(every * inv);
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) d.p[i] = __fmul2_rn(d.p[i], __ffma2_rn(f.p[i], x, y));
+      for (int i = 0; i < V / 2; ++i) d.p[i] = __fmul2_rn(d.p[i], __ffma2_rn(f(i), x, y));
     } else {
       Row<V> ds;
       float2 ns2 = both(0.f), fs = both(0.f);
       row_sigmoid(v, d, mx, mxl, [&](int i, float2 s, float2 slope) {
         ns2 = __fadd2_rn(ns2, s);
-        fs = __ffma2_rn(f.p[i], s, fs);
+        fs = __ffma2_rn(f(i), s, fs);
         ds.p[i] = slope;
       });
       const float norm = group_sum<G>(ns2.x + ns2.y), fq = group_sum<G>(fs.x + fs.y);
@@ -876,19 +874,54 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>(tru
       const float2 x = both(qi), y = both(-fq * qi * qi), w2 = both(zl);
 #pragma unroll
       for (int i = 0; i < V / 2; ++i)
-        d.p[i] = __ffma2_rn(ds.p[i], __ffma2_rn(f.p[i], x, y), __fmul2_rn(d.p[i], w2));
-    }
-    if (p.d_weights) {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) d.p[i] = __fadd2_rn(d.p[i], reinterpret_cast<const float2*>(row + e0)[i]);
-      __syncwarp();
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        if (id[s] >= 0) row[id[s]] = 0.f;
-      __syncwarp();
+        d.p[i] = __ffma2_rn(ds.p[i], __ffma2_rn(f(i), x, y), __fmul2_rn(d.p[i], w2));
     }
     if (!keep) row_fill(d, 0.f);
-    if (inside) row_put(p.d_logits, p.type, p.vec_out, t * E, e0, E, d);
+    if (!WEIGHTS && p.type != kElemF32 && p.vec_out == 8) {
+      // Nothing to add, and a lane's 16 or 32 bytes are whole sectors or
+      // halves that its next store fills: straight out (47 us against 54
+      // through shared memory at T = 131072, E = 256).
+#pragma unroll
+      for (int c = 0; c < V; c += 8) {
+        const float2* x = d.p + c / 2;
+        if (inside && e0 + c < E)
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.d_logits) + t * E + e0 + c) =
+              make_uint4(pack16(x[0].x, x[0].y, p.type), pack16(x[1].x, x[1].y, p.type),
+                         pack16(x[2].x, x[2].y, p.type), pack16(x[3].x, x[3].y, p.type));
+      }
+      continue;
+    }
+    __syncwarp();  // the last step's rows are stored
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q)
+      fours[four_at<V>(lane, q)] = make_float4(d.p[2 * q].x, d.p[2 * q].y, d.p[2 * q + 1].x, d.p[2 * q + 1].y);
+    __syncwarp();
+    if constexpr (WEIGHTS) {
+      const float off = p.normalize ? dot : 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        g[s] = w[s] * (g[s] - off);
+        // Slots of one expert (the caller's choice may repeat it) are added
+        // in slot order by the lowest of their lanes.
+        const int l = lane / G * G + id[s] / V;
+        const int key = id[s] >= 0 ? l * V + id[s] % V : -1 - lane;
+        const uint32_t peers = __match_any_sync(0xffffffffu, key);
+        bool mine = true;
+        if (__any_sync(0xffffffffu, peers != 1u << lane)) {
+          float sum = 0.f;
+          for (int x = 0; x < 32; ++x) {
+            const float other = __shfl_sync(0xffffffffu, g[s], x);
+            if (peers >> x & 1u) sum += other;
+          }
+          g[s] = sum;
+          mine = lane == __ffs(peers) - 1;
+        }
+        if (id[s] >= 0 && mine && keep)
+          reinterpret_cast<float*>(fours + four_at<V>(l, id[s] % V / 4))[id[s] % 4] += g[s];
+        __syncwarp();
+      }
+    }
+    rows_store<G, V>(fours, p.d_logits, p.type, p.vec_out, base, hi, E, lane);
   }
 }
 
