@@ -221,6 +221,64 @@ def test_route_long_batches(T, E, k):
     assert torch.all((d.double() - ref).abs() <= 8 * (span + 80 + E / 8) * U * mag)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,E,k,sequences", [(12000, 256, 8, 3), (6000, 1000, 4, 2), (50000, 16, 2, 5), (2400, 64, 6, 800)])
+def test_route_long_sequences(T, E, k, sequences, scoring):
+    """Several sequences of many blocks each (and many of few), padded: losses and counts against float64 torch."""
+    x, _ = _logits(T, E, torch.float32, T)
+    L = T // sequences
+    mask = torch.arange(L, device=DEV)[None] < torch.linspace(0, 1.2, sequences, device=DEV)[:, None] * L
+    r = router.route_forward_train(x, k, mask=mask, sequences=sequences, scoring=scoring)
+    keep = mask.reshape(T)
+    s = torch.softmax(x.double(), 1) if scoring == "softmax" else torch.sigmoid(x.double())
+    q = torch.where(keep[:, None], s / s.sum(1, keepdim=True), 0).view(sequences, L, E).sum(1)
+    seq = (torch.arange(T, device=DEV) // L)[:, None] * E
+    c = torch.bincount((seq + r.ids.long())[keep].reshape(-1), minlength=sequences * E).view(sequences, E)
+    n = keep.view(sequences, L).sum(1)
+    assert torch.equal(r.counts.long(), c) and torch.equal(r.tokens.long(), n) and torch.all(r.ids[~keep] == -1)
+    nn = n.clamp(min=1).double()[:, None]
+    want = float((c * E / (k * nn) * q / nn).sum() / (n > 0).sum())
+    lse = torch.logsumexp(x.double(), 1)[keep]
+    span = float(x.max() - x.min()) + float(x.abs().max())
+    tol = (2 * (span + 80) + T / 1000 + 50) * U                    # see test_route_long_batches
+    assert abs(r.balance_loss.item() - want) <= tol * want
+    assert abs(r.z_loss.item() - float((lse ** 2).mean())) <= 2 * tol * float((lse ** 2 + lse.abs()).mean())
+
+
+@pytest.mark.parametrize("scoring,normalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("E,k", [(8, 8), (20, 16), (40, 3), (130, 16)])
+def test_route_given_repeats(E, k, scoring, normalize):
+    """One expert several times in a row, in neighbouring slots and in slots that one lane holds."""
+    x, dw = _logits(60, E, torch.float32, E + k)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(k)
+    ids = torch.randint(0, min(E, 4), (60, k), generator=g, device=DEV, dtype=torch.int32)
+    ids[::3] = ids[::3, :1]
+    dw = torch.randn((60, k), generator=g, device=DEV)
+    _check_route(x, k, dw, ids=ids, scoring=scoring, normalize=normalize)
+    r = router.route_forward_train(x, k, ids=ids, scoring=scoring, normalize=normalize)
+    a, b = (router.route_backward(x, r, d_weights=dw, scoring=scoring, normalize=normalize) for _ in range(2))
+    assert torch.equal(a, b)
+
+
+def test_route_two_streams_at_once():
+    """Calls that overlap on two streams, each with workspaces and counters of its own."""
+    xs = [_logits(30000, 256, torch.float32, 20)[0], _logits(20000, 128, torch.bfloat16, 21)[0]]
+    want = [router.route_forward_train(x, 8) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(router.route_forward_train(xs[i], 8))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(a, b)
+
+
 def test_route_on_another_stream_and_in_a_graph():
     x, dw = _logits(500, 64, torch.float32, 10)
     how = {"sequences": 5, "scoring": "sigmoid"}
