@@ -522,12 +522,17 @@ __device__ __forceinline__ void route_finish(const RouteParams& p, int64_t seq, 
   }
 }
 
-// Blocks per SM that the register budget is cut for.
+// Blocks per SM that the register budget is cut for.  E = 1024, T = 32768, f32,
+// forward: 139 us at one block of 190 registers a thread, 83 at two of 128;
+// E = 256, T = 131072: no gain from a fourth block at 64 (spills).
 template <int G, int V, int KMAX>
 constexpr int route_residents() {
   return V == 32 ? 2 : (KMAX + G - 1) / G <= 4 ? 3 : 2;
 }
 
+// T = 131072, E = 256, k = 8, f32: 98 us; with given experts, bf16, sigmoid 62
+// (HBM's share 22 and 11).  Bounded by instruction issue, half of its slots at
+// 24 warps an SM, and by the special-function pipe.
 template <int G, int V, int KMAX>
 __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_train_kernel(const RouteParams p) {
   constexpr int TPW = 32 / G;                // tokens per warp and step
@@ -879,8 +884,8 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     if (!keep) row_fill(d, 0.f);
     if (!WEIGHTS && p.type != kElemF32 && p.vec_out == 8) {
       // Nothing to add, and a lane's 16 or 32 bytes are whole sectors or
-      // halves that its next store fills: straight out (47 us against 54
-      // through shared memory at T = 131072, E = 256).
+      // halves that its next store fills: straight out (45 us against 54
+      // through shared memory at T = 131072, E = 256, sigmoid).
 #pragma unroll
       for (int c = 0; c < V; c += 8) {
         const float2* x = d.p + c / 2;

@@ -105,7 +105,6 @@ class RouteTrain(NamedTuple):
 
 _ELEMS = {torch.float32: _lib.MOE_ELEM_F32, torch.bfloat16: _lib.MOE_ELEM_BF16, torch.float16: _lib.MOE_ELEM_F16}
 _SCORING = {"softmax": 0, "sigmoid": 1}
-_ROUTED_TYPES = (torch.int32, torch.float32, torch.int32, torch.int32)  # ids, weights, counts, tokens
 
 
 def _elem(t: torch.Tensor, name: str) -> int:
@@ -260,14 +259,15 @@ def route_backward(logits: torch.Tensor, routed: RouteTrain, *, d_weights: Optio
     logits, code, ld, mask_ptr, how, mask = _route_args(logits, mask, sequences, scoring)
     dev = logits.device
     T, E = logits.shape
-    ids, weights, counts, tokens = saved = routed[:4]
+    ids, weights, counts, tokens = routed[:4]
     k = ids.shape[-1]
     if (ids.shape != (T, k) or weights.shape != (T, k) or counts.shape != (sequences, E) or tokens.shape != (sequences,)
-            or ids.device != dev):
+            or not ids.get_device() == weights.get_device() == counts.get_device() == tokens.get_device() == dev.index):
         raise ValueError(f"routed has ids {tuple(ids.shape)}, weights {tuple(weights.shape)}, counts "
                          f"{tuple(counts.shape)} and tokens {tuple(tokens.shape)} on {ids.device}, expected {(T, k)}, "
                          f"{(T, k)}, {(sequences, E)} and {(sequences,)} on {dev}")
-    if tuple(t.dtype for t in saved) != _ROUTED_TYPES or not all(map(torch.Tensor.is_contiguous, saved)):
+    if not (ids.dtype == counts.dtype == tokens.dtype == torch.int32 and weights.dtype == torch.float32
+            and ids.is_contiguous() and weights.is_contiguous() and counts.is_contiguous() and tokens.is_contiguous()):
         raise TypeError("routed's tensors must be as route_forward_train returns them: int32 and float32, contiguous")
     if d_weights is not None:
         if d_weights.shape != (T, k) or d_weights.device != dev:
