@@ -1,4 +1,6 @@
-"""Builds ``libmoe_b200.so`` (sm_100a) from the CUDA sources in this folder.
+"""Builds ``libmoe_b200.so`` (sm_100a) from the CUDA sources in this folder, and
+the CPython binding of the layer-training entry points (``layer_binding.cpp``,
+against the installed torch's headers).
 
 Output: ``<package>/lib/libmoe_b200.so``.  nvcc cross-compiles for sm_100a
 without a GPU.  The build is skipped when the library is newer than every
@@ -11,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -66,6 +69,39 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
+def native_path() -> Path:
+    import torch
+    return LIB_DIR / f"moe_layer_native.{sys.implementation.cache_tag}-torch{torch.__version__}.so"
+
+
+def build_native(force: bool = False) -> Path:
+    """The binding ``src/_lib.py::native`` loads; one per Python and torch version."""
+    import torch
+    out, src = native_path(), CSRC / "layer_binding.cpp"
+    inputs = [src, REPO / "include" / "moe_b200.h"]
+    if out.exists() and not force and all(p.stat().st_mtime <= out.stat().st_mtime for p in inputs):
+        return out
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    dirs = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+            REPO / "include"]
+    tmp = out.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-fPIC", "-shared", "-std=c++17",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"]]
+    for d in dirs:
+        cmd += ["-isystem", str(d)]
+    cmd += [str(src), "-o", str(tmp), "-L", str(root / "lib")]
+    # The shared C++ library by name: a compiler set up to link it statically
+    # would give the module streams of its own, apart from those torch set up.
+    cmd += ["-l:libstdc++.so.6"]
+    cmd += [f"-l{name}" for name in ("torch_python", "torch_cuda", "torch_cpu", "torch", "c10_cuda", "c10")]
+    subprocess.run(cmd, check=True, cwd=str(CSRC))
+    os.replace(tmp, out)
+    return out
+
+
 if __name__ == "__main__":
     out = build(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(out)
+    print(build_native(force="--force" in sys.argv))

@@ -1,13 +1,17 @@
 """ctypes binding of ``libmoe_b200.so`` (declarations: include/moe_b200.h).
 
 There is no fallback: if the library is missing or fails to load, every
-entry point raises.
+entry point raises.  The layer-training entry points have a CPython binding of
+their own (:func:`native`), which calls the same library.
 """
 
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
+import sys
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libmoe_b200.so"
@@ -182,6 +186,36 @@ def lib() -> ctypes.CDLL:
     L.moe_ep_destroy.restype = ctypes.c_int
     _lib = L
     return L
+
+
+_native = None
+
+
+def native_path() -> Path:
+    """The layer-training entry points' binding, built for this Python and torch."""
+    import torch
+    return LIB_PATH.parent / f"moe_layer_native.{sys.implementation.cache_tag}-torch{torch.__version__}.so"
+
+
+def native():
+    """Loads the binding once (csrc/layer_binding.cpp) and hands it the
+    library's functions; raises if it is absent."""
+    global _native
+    if _native is not None:
+        return _native
+    L, path = lib(), native_path()
+    if not path.exists():
+        raise RuntimeError(f"{path} not found: build it with `python __graft_entry__.py` or "
+                           f"`python pallas-moe-kernel_b200/csrc/build.py`")
+    loader = importlib.machinery.ExtensionFileLoader("moe_layer_native", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("moe_layer_native", loader))
+    loader.exec_module(module)
+    names = ("moe_route_train_workspace_size", "moe_route_train_counters", "moe_route_train", "moe_route_backward",
+             "moe_combine_rows_backward", "moe_gather_rows_backward", "moe_grad_norm_workspace_size", "moe_grad_norm",
+             "moe_clip_grads", "moe_last_error")
+    module.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names}, MoeError)
+    _native = module
+    return module
 
 
 def check(code: int) -> None:
