@@ -25,14 +25,16 @@ static int route_lanes(int E) {
   return g;
 }
 
-// Blocks per sequence: enough that a warp has one step of tokens, and at most
-// as many over all sequences as are resident (3 an SM at 80 registers a thread,
-// 2 at 128): a second, short wave costs its whole length.
-static int64_t route_blocks(int E) { return 148 * (E > 512 ? 2 : 3); }
+// Blocks per sequence: one for every step (a token per row group of the block)
+// while all of them are resident (3 blocks an SM at 80 registers a thread, 2 at
+// 128), else as few as share the steps evenly: a block with one token more than
+// its neighbours, or a second, short wave, costs a whole step.
 static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
   const int64_t step = kRouteWarps * (32 / route_lanes(E));
-  const int64_t most = std::max<int64_t>(1, route_blocks(E) / std::max<int64_t>(1, sequences));
-  return std::max<int64_t>(1, std::min((seq_len + step - 1) / step, most));
+  const int64_t steps = std::max<int64_t>(1, (seq_len + step - 1) / step);
+  const int64_t resident = std::max<int64_t>(1, 148 * (E > 512 ? 2 : 3) / std::max<int64_t>(1, sequences));
+  const int64_t each = (steps + resident - 1) / resident;
+  return (steps + each - 1) / each;
 }
 
 struct RouteSpace {

@@ -397,6 +397,49 @@ __host__ __device__ __forceinline__ int route_groups(int64_t chunks, int E) {
   return chunks * E > 8 * kRouteThreads ? (int)((chunks + kRouteGroup - 1) / kRouteGroup) : 1;
 }
 
+// Tokens of a block: whole steps of the block, the last one takes what is left.
+__device__ __forceinline__ int64_t route_share(int64_t seq_len, int chunks, int step) {
+  const int64_t steps = (seq_len + step - 1) / step;
+  return (steps + chunks - 1) / chunks * step;
+}
+
+// The end of a sequence, by one block whose threads hold parts of
+// sum_e c_e sum_t q_te, sum lse^2 and the number of tokens; the block that
+// ends the last sequence ends the call.
+__device__ __forceinline__ void route_close(const RouteParams& p, int64_t seq, double sum, double z, double n,
+                                            uint32_t* counter, double* s_w, int* s_flag) {
+  const int E = p.E, tid = threadIdx.x;
+  const int64_t b0 = seq * p.chunks;
+  block_sum3(sum, z, n, s_w);
+  if (tid == 0) {
+    p.tokens[seq] = (int)n;
+    sum = n > 0.0 ? sum * E / (p.k * n * n) : 0.0;
+    if (p.S == 1) {
+      *p.balance = (float)sum;
+      *p.z = (float)(n > 0.0 ? z / n : 0.0);
+    } else {
+      p.seq_part[seq] = sum;
+      p.part_z[b0] = z;
+    }
+  }
+  if (p.S == 1 || !last_block(counter, p.S, s_flag)) return;
+  double bal = 0.0, live = 0.0;
+  z = n = 0.0;
+  for (int64_t i = tid; i < p.S; i += kRouteThreads) {
+    const int ns = __ldcg(p.tokens + i);
+    bal += __ldcg(p.seq_part + i);
+    z += __ldcg(p.part_z + i * p.chunks);
+    n += ns;
+    live += ns > 0;
+  }
+  live = block_sum(live, s_w);
+  block_sum3(bal, z, n, s_w);
+  if (tid == 0) {
+    *p.balance = (float)(live > 0.0 ? bal / live : 0.0);
+    *p.z = (float)(n > 0.0 ? z / n : 0.0);
+  }
+}
+
 // Adds up blocks' sums, as far as this block is the last one to finish.
 __device__ __forceinline__ void route_finish(const RouteParams& p, int64_t seq, int chunk, double* s_w, double* s_q, int* s_c,
                                              int* s_flag) {
@@ -492,34 +535,7 @@ __device__ __forceinline__ void route_finish(const RouteParams& p, int64_t seq, 
       sum = (double)c * q;
     }
   }
-  block_sum3(sum, z, n, s_w);
-  if (tid == 0) {
-    p.tokens[seq] = (int)n;
-    sum = n > 0.0 ? sum * E / (p.k * n * n) : 0.0;
-    if (p.S == 1) {
-      *p.balance = (float)sum;
-      *p.z = (float)(n > 0.0 ? z / n : 0.0);
-    } else {
-      p.seq_part[seq] = sum;
-      p.part_z[b0] = z;
-    }
-  }
-  if (p.S == 1 || !last_block(seq_counters + p.S, p.S, s_flag)) return;
-  double bal = 0.0, live = 0.0;
-  z = n = 0.0;
-  for (int64_t i = tid; i < p.S; i += kRouteThreads) {
-    const int ns = __ldcg(p.tokens + i);
-    bal += __ldcg(p.seq_part + i);
-    z += __ldcg(p.part_z + i * p.chunks);
-    n += ns;
-    live += ns > 0;
-  }
-  live = block_sum(live, s_w);
-  block_sum3(bal, z, n, s_w);
-  if (tid == 0) {
-    *p.balance = (float)(live > 0.0 ? bal / live : 0.0);
-    *p.z = (float)(n > 0.0 ? z / n : 0.0);
-  }
+  route_close(p, seq, sum, z, n, seq_counters + p.S, s_w, s_flag);
 }
 
 // Blocks per SM that the register budget is cut for.  E = 1024, T = 32768, f32,
@@ -556,8 +572,9 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
 
   const int64_t seq = blockIdx.x / p.chunks;
   const int chunk = blockIdx.x % p.chunks;
-  const int64_t lo = seq * p.seq_len + p.seq_len * chunk / p.chunks;
-  const int64_t hi = seq * p.seq_len + p.seq_len * (chunk + 1) / p.chunks;
+  const int64_t per = route_share(p.seq_len, p.chunks, kRouteWarps * TPW);
+  const int64_t lo = seq * p.seq_len + chunk * per;
+  const int64_t hi = seq * p.seq_len + min(p.seq_len, (chunk + 1) * per);
   Row<V> acc;
   row_fill(acc, 0.f);
   float z = 0.f;
@@ -707,7 +724,7 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     n += __shfl_xor_sync(0xffffffffu, n, o);
   }
   float* s_q = reinterpret_cast<float*>(s_quads);
-  __syncthreads();
+  __syncthreads();  // the rows in work are done with
   if (lane < G) {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
@@ -720,6 +737,20 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     s_n[warp] = n;
   }
   __syncthreads();
+  if (p.chunks == 1) {  // a sequence of its own: nothing to wait for, nothing by way of memory
+    const int tid = threadIdx.x;
+    double sum = 0.0;
+    for (int e = tid; e < E; e += kRouteThreads) {
+      float qs = 0.f;
+#pragma unroll
+      for (int w = 0; w < kRouteWarps; ++w) qs += s_q[w * (G * V) + e];
+      p.counts[seq * E + e] = s_cnt[e];
+      sum += (double)s_cnt[e] * (double)qs;
+    }
+    route_close(p, seq, sum, tid < kRouteWarps ? s_z[tid] : 0.0, tid < kRouteWarps ? s_n[tid] : 0,
+                p.counters + 2 * (int64_t)p.S, s_w, &s_flag);
+    return;
+  }
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
     float sum = 0.f;
 #pragma unroll
@@ -774,9 +805,14 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
   const int e0 = gl * V, E = p.E, k = p.k;
   const int64_t seq = blockIdx.x / p.chunks;
   const int chunk = blockIdx.x % p.chunks;
-  const int64_t lo = seq * p.seq_len + p.seq_len * chunk / p.chunks;
-  const int64_t hi = seq * p.seq_len + p.seq_len * (chunk + 1) / p.chunks;
+  const int64_t per = route_share(p.seq_len, p.chunks, kRouteWarps * TPW);
+  const int64_t lo = seq * p.seq_len + chunk * per;
+  const int64_t hi = seq * p.seq_len + min(p.seq_len, (chunk + 1) * per);
   float4* fours = s_rows[warp];
+  {  // the first rows come while the experts' factors are made
+    const int64_t t = lo + warp * TPW + lane / G;
+    row_prefetch<V>(p.logits, p.type, t * p.ld, e0, E, t < hi);
+  }
 
   // Tokens in all sequences and sequences with any.
   const int ns = __ldg(p.tokens + seq);
