@@ -23,6 +23,7 @@
 // 2^-46 of its square.)  No atomics: a result repeats bit for bit.
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "router_train.cuh"
@@ -37,10 +38,10 @@ constexpr int kNormBlocksPerSm = 4;
 // itself.  Above that (155 MB of input) a block takes one unit and the hardware
 // hands them out: with resident blocks in a fixed order, the slowest of them
 // set the pace (scaling 2 x 470 M f32 to bf16: 951 us on 592 blocks, 838 on
-// 9472, 798 with one unit each; below, the third launch costs what that
-// gives: 30 M bf16 33 us in two launches and 40 in three, 60 M 64 and 67, 120 M
-// 126 and 123).  A norm's blocks are kept to as many partials
-// as one block then adds up in a few microseconds.
+// 9472, 798 with one unit each; below, the third launch costs what that gives:
+// three launches ran 30 M bf16 21% slower than two, 60 M 5% slower, 120 M 2%
+// faster).  A norm's blocks are kept to as many partials as one block then adds
+// up in a few microseconds.
 constexpr int kNormResident = 148 * kNormBlocksPerSm;
 constexpr uint32_t kNormLarge = 8 * kNormResident;
 constexpr int kNormMaxBlocks = 16384;
@@ -120,10 +121,12 @@ __device__ __forceinline__ const uint4* chunk_ptr(const void* p, int64_t i) {
 }
 
 // A block's pass over one unit: all of a thread's chunks are loaded, then
-// chunks(raw, index of the first, number in the tensor) takes them (zeros past
-// the end); single(in offset, out offset) takes the elements outside chunks:
+// chunks(raw, index of the first, number in the tensor, whether the tensor is
+// dense and the unit whole) takes them (zeros past the end); single(in offset, out offset) takes the elements outside chunks:
 // those before and after (in a tensor's first unit), or all where head < 0.
-template <int TYPE, class Chunks, class Single>
+// WHOLE: whole units have a body of their own (the scaling: 41 -> 39 us for 60 M
+// bf16; the norm's sums, twice in one kernel, spill: 27 -> 40 us).
+template <int TYPE, bool WHOLE, class Chunks, class Single>
 __device__ __forceinline__ void walk_unit(const GradEntry& e, int64_t u, Chunks&& chunks, Single&& single) {
   constexpr int CE = chunk_elems(TYPE);
   const int64_t rows = e.rows, cols = e.cols, total = rows * cols;
@@ -136,7 +139,13 @@ __device__ __forceinline__ void walk_unit(const GradEntry& e, int64_t u, Chunks&
   const int64_t n = (total - e.head) / CE;  // chunks
   const int64_t first = u * (kNormThreads * kNormChunks) + threadIdx.x;
   uint4 raw[kNormChunks];
-  if (rows == 1) {
+  const bool whole = WHOLE && rows == 1 && (u + 1) * (kNormThreads * kNormChunks) <= n;
+  if (whole) {  // most units: nothing to ask per chunk
+    const uint4* q = chunk_ptr<TYPE>(e.in, e.head) + first;
+#pragma unroll
+    for (int s = 0; s < kNormChunks; ++s) raw[s] = q[s * kNormThreads];
+    chunks(raw, first, n, std::true_type());
+  } else if (rows == 1) {
     const uint4* q = chunk_ptr<TYPE>(e.in, e.head) + first;
 #pragma unroll
     for (int s = 0; s < kNormChunks; ++s)
@@ -148,7 +157,7 @@ __device__ __forceinline__ void walk_unit(const GradEntry& e, int64_t u, Chunks&
                    ? *chunk_ptr<TYPE>(e.in, entry_at((first + s * kNormThreads) * CE, rows, cols, e.in_ld))
                    : make_uint4(0, 0, 0, 0);
   }
-  chunks(raw, first, n);
+  if (!whole) chunks(raw, first, n, std::false_type());
   if (u == 0) {
     const int64_t tail = e.head + CE * n;
     const int64_t i = threadIdx.x < 8 ? (int64_t)threadIdx.x : tail + threadIdx.x - 8;
@@ -194,9 +203,9 @@ __device__ __forceinline__ void norm_add(const float (&v)[N], NormAcc& acc) {
 template <int NORM, int TYPE>
 __device__ __forceinline__ void norm_unit(const GradEntry& e, int64_t u, NormAcc& acc) {
   constexpr int CE = chunk_elems(TYPE), PER = 32 / CE;  // chunks of 32 elements
-  walk_unit<TYPE>(
+  walk_unit<TYPE, false>(
       e, u,
-      [&](const uint4 (&raw)[kNormChunks], int64_t, int64_t) {
+      [&](const uint4 (&raw)[kNormChunks], int64_t, int64_t, auto) {
 #pragma unroll
         for (int s = 0; s < kNormChunks; s += PER) {
           float v[32];
@@ -270,18 +279,18 @@ template <int IN, int OUT>
 __device__ __forceinline__ void clip_unit(const GradEntry& e, int64_t u, float coef) {
   constexpr int CE = chunk_elems(IN);
   const int64_t rows = e.rows;
-  walk_unit<IN>(
+  walk_unit<IN, true>(
       e, u,
-      [&](const uint4 (&raw)[kNormChunks], int64_t first, int64_t n) {
+      [&](const uint4 (&raw)[kNormChunks], int64_t first, int64_t n, auto whole) {
 #pragma unroll
         for (int s = 0; s < kNormChunks; ++s) {
           const int64_t c = first + s * kNormThreads;
-          if (c >= n) continue;
+          if (!decltype(whole)::value && c >= n) continue;
           float v[CE];
           chunk_values<IN>(raw[s], v);
 #pragma unroll
           for (int x = 0; x < CE; ++x) v[x] *= coef;
-          const int64_t at = rows == 1 ? e.head + c * CE : entry_at(c * CE, rows, e.cols, e.out_ld);
+          const int64_t at = decltype(whole)::value || rows == 1 ? e.head + c * CE : entry_at(c * CE, rows, e.cols, e.out_ld);
           if (OUT == kElemF32) {
 #pragma unroll
             for (int x = 0; x < CE; x += 4)
