@@ -40,7 +40,8 @@ static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
 struct RouteSpace {
   size_t q, c, z, n, seq, bytes;
 };
-static RouteSpace route_space(int64_t blocks, int64_t sequences, int E) {
+static RouteSpace route_space(int64_t chunks, int64_t sequences, int E) {
+  const int64_t blocks = chunks * sequences, sums = chunks > 1 ? blocks : 0;  // one block: nothing to hand over
   RouteSpace s;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -48,8 +49,8 @@ static RouteSpace route_space(int64_t blocks, int64_t sequences, int E) {
     at += align256(bytes);
     return here;
   };
-  s.q = take((size_t)blocks * E * sizeof(float));
-  s.c = take((size_t)blocks * E * sizeof(int32_t));
+  s.q = take((size_t)sums * E * sizeof(float));
+  s.c = take((size_t)sums * E * sizeof(int32_t));
   s.z = take((size_t)blocks * sizeof(double));
   s.n = take((size_t)blocks * sizeof(int32_t));
   s.seq = take((size_t)sequences * sizeof(double));
@@ -379,7 +380,7 @@ int64_t moe_route_train_counters(int64_t T, int32_t E, int64_t sequences) {
 
 size_t moe_route_train_workspace_size(int64_t T, int32_t E, int64_t sequences) {
   if (T < 0 || E < 1 || E > kRouteMaxExperts || sequences < 1 || T % sequences) return 0;
-  return route_space(route_chunks(T / sequences, sequences, E) * sequences, sequences, E).bytes;
+  return route_space(route_chunks(T / sequences, sequences, E), sequences, E).bytes;
 }
 
 int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T, int32_t E, int32_t k,
@@ -401,7 +402,7 @@ int moe_route_train(const void* logits, int32_t elem_type, int64_t ld, int64_t T
   if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(elem_type))
     return fail(MOE_ERR_MISALIGNED, "logits are not aligned to their elements");
   const int64_t seq_len = T / sequences, chunks = route_chunks(seq_len, sequences, E), blocks = chunks * sequences;
-  const RouteSpace s = route_space(blocks, sequences, E);
+  const RouteSpace s = route_space(chunks, sequences, E);
   if (!workspace || workspace_bytes < s.bytes)
     return fail(MOE_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes < required %zu", workspace_bytes, s.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u)

@@ -282,17 +282,31 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // e_i = 2^(l_i log2 e - mxl), mxl = the row maximum times log2 e, rounded: one
 // factor near 1 in all of them, which the ratios p = e / sum(e) and
 // lse = (mxl + log2 sum(e)) ln 2 are free of.  Rows that are not kept have
-// l = -inf throughout, and e = 0.
+// l = -inf throughout, mx = 0 and e = 0.  Where mx log2 e leaves the f32 range
+// (a row masked throughout by the type's lowest value), the maximum is taken
+// off first.
+__device__ __forceinline__ bool far_out(float mx) { return fabsf(mx) > 1e38f; }
 template <int V>
-__device__ __forceinline__ float row_exp(const Row<V>& v, float mxl, Row<V>& e) {
+__device__ __forceinline__ float row_exp(const Row<V>& v, float mx, float mxl, Row<V>& e) {
   float2 total = both(0.f);
+  if (far_out(mx)) {
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) {
-    const float2 x = __ffma2_rn(v.p[i], both(kLog2e), both(-mxl));
-    e.p[i] = make_float2(ex2_ftz(x.x), ex2_ftz(x.y));
-    total = __fadd2_rn(total, e.p[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      e.p[i] = make_float2(ex2_ftz((v.p[i].x - mx) * kLog2e), ex2_ftz((v.p[i].y - mx) * kLog2e));
+      total = __fadd2_rn(total, e.p[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 x = __ffma2_rn(v.p[i], both(kLog2e), both(-mxl));
+      e.p[i] = make_float2(ex2_ftz(x.x), ex2_ftz(x.y));
+      total = __fadd2_rn(total, e.p[i]);
+    }
   }
   return total.x + total.y;
+}
+__device__ __forceinline__ float row_lse(float mx, float mxl, float total) {
+  return far_out(mx) ? fmaf(lg2_ftz(total), kLn2, mx) : (mxl + lg2_ftz(total)) * kLn2;
 }
 
 // Sigmoid scores from the same exponentials.  For a maximum mx >= 0,
@@ -326,7 +340,7 @@ __device__ __forceinline__ void row_sigmoid(const Row<V>& v, const Row<V>& e, fl
 // The score of a chosen logit relative to `top`: e^(l - top), or a sigmoid
 // times e^-min(top, 0).
 __device__ __forceinline__ float slot_score(float l, float top, bool sigmoid) {
-  if (!sigmoid) return ex2_ftz((l - top) * kLog2e);
+  if (!sigmoid) return ex2_ftz((l - top) * kLog2e);  // normalised: top is one of the row's chosen
   const float m = fminf(top, 0.f);
   return rcp_ftz(ex2_ftz(m * kLog2e) + ex2_ftz((m - l) * kLog2e));
 }
@@ -546,7 +560,7 @@ constexpr int route_residents() {
   return V == 32 ? 2 : (KMAX + G - 1) / G <= 4 ? 3 : 2;
 }
 
-// T = 131072, E = 256, k = 8, f32: 98 us; with given experts, bf16, sigmoid 62
+// T = 131072, E = 256, k = 8, f32: 101 us; with given experts, bf16, sigmoid 62
 // (HBM's share 22 and 11).  Bounded by instruction issue, half of its slots at
 // 24 warps an SM, and by the special-function pipe.
 template <int G, int V, int KMAX>
@@ -604,8 +618,8 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     if (!keep) row_fill(v, -INFINITY);  // a row of NaN takes no part either
     const float mxl = keep ? mx * kLog2e : 0.f;
     Row<V> ex;
-    const float total = group_sum<G>(row_exp(v, mxl, ex));
-    const float lse = keep ? (mxl + lg2_ftz(total)) * kLn2 : 0.f;
+    const float total = group_sum<G>(row_exp(v, keep ? mx : 0.f, mxl, ex));
+    const float lse = keep ? row_lse(mx, mxl, total) : 0.f;
     z += lse * lse;
     n += keep;
     float inv;  // 1 / the sum of the scores
@@ -691,7 +705,13 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       // -inf: no expert in this slot, or one chosen by the caller with score 0.
-      w[s] = keep && sel[s] > -INFINITY ? slot_score(sel[s], top, p.sigmoid) : 0.f;
+      w[s] = 0.f;
+      if (keep && sel[s] > -INFINITY) {
+        // A plain softmax probability is one of the row's e over their sum,
+        // mxl's rounding included (at |mx| = 65504 that is 2e-3).
+        if (!p.sigmoid && !p.normalize && !far_out(mx)) w[s] = ex2_ftz(fmaf(sel[s], kLog2e, -mxl));
+        else w[s] = slot_score(sel[s], top, p.sigmoid);
+      }
       if (sel[s] != sel[s]) w[s] = sel[s];
       sum += w[s];
     }
@@ -883,7 +903,7 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
     const bool keep = mx > -INFINITY;
     const float mxl = keep ? mx * kLog2e : 0.f;
     Row<V> d;
-    float total = row_exp(v, mxl, d);
+    float total = row_exp(v, keep ? mx : 0.f, mxl, d);
     if (WEIGHTS) dot = group_sum<G>(dot);
     if (!p.sigmoid) {
       float2 fs = both(0.f);
@@ -893,7 +913,7 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
       const float fq = group_sum<G>(fs.x + fs.y);
       const float inv = keep ? rcp_ftz(total) : 0.f;
       // A row's share of every p: the z loss, the centring, the weights' dot.
-      const float every = dz * ((mxl + lg2_ftz(total)) * kLn2) - fq * inv - (p.normalize ? 0.f : dot);
+      const float every = dz * row_lse(mx, mxl, total) - fq * inv - (p.normalize ? 0.f : dot);
       const float2 x = both(inv), y = both(every * inv);
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) d.p[i] = __fmul2_rn(d.p[i], __ffma2_rn(f(i), x, y));
@@ -910,7 +930,7 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
       float zl = 0.f;
       if (p.d_z) {
         total = group_sum<G>(total);
-        zl = keep ? dz * ((mxl + lg2_ftz(total)) * kLn2) * rcp_ftz(total) : 0.f;
+        zl = keep ? dz * row_lse(mx, mxl, total) * rcp_ftz(total) : 0.f;
       }
       const float2 x = both(qi), y = both(-fq * qi * qi), w2 = both(zl);
 #pragma unroll

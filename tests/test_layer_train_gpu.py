@@ -151,6 +151,28 @@ def test_route_lowest_value_and_single_parts():
     assert torch.all(router.route_backward(y, r) == 0)
 
 
+@pytest.mark.parametrize("scoring,normalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_route_rows_of_the_lowest_value(dtype, scoring, normalize):
+    """Rows masked throughout by the type's lowest value are rows of equal logits; their product with log2 e is not finite."""
+    x, dw = _logits(48, 20, dtype, 14)
+    x[5] = torch.finfo(dtype).min
+    x[6] = torch.finfo(dtype).min
+    x[6, 7] = 0.5
+    x[7] = torch.finfo(dtype).max / 2
+    dw = dw[:, :4]
+    r = router.route_forward_train(x, 4, scoring=scoring, normalize=normalize)
+    d = router.route_backward(x, r, d_weights=dw, d_balance=torch.ones((), device=DEV), scoring=scoring,
+                              normalize=normalize)
+    ref = orc.route_train(_np(x), 4, scoring=scoring, normalize=normalize)
+    refd, scale = orc.route_train_backward(ref, _np(dw), 1.0)
+    assert np.array_equal(r.ids.cpu().numpy(), ref["ids"]) and r.tokens.item() == 48
+    # Arguments of exp up to 15 from the maximum (others vanish in 64 bits too): as in _check_route, 2 (15 + 80 + k) u.
+    _close(r.weights, ref["weights"], 2 * 100 * U * ref["weights"] + 2.0 ** -126)
+    assert abs(r.balance_loss.item() - ref["balance"]) <= 2 * 160 * U * ref["balance"]
+    _close(d, refd, 4 * 120 * U * scale + 1e-37, dtype)
+
+
 def test_route_nan_is_never_chosen_and_reaches_the_losses():
     x, _ = _logits(32, 8, torch.float32, 6)
     x[5, 2] = float("nan")
