@@ -12,8 +12,8 @@
 // 4-element vectors (16 bytes of f32, 8 of the 16-bit types); dot products are
 // summed in f32 per thread and then across the threads in a fixed order.
 // Measured against the 6547 GB/s of a copy: combine at T = 8192, k = 8,
-// D = 7168 (f32, bf16 out) 466 us = 1.00, gather at T = 16384, k = 2, D = 4096
-// (f32, bf16 out) 99 us = 1.03.
+// D = 7168 (f32, bf16 out) 466 to 476 us = 0.98 to 1.00, gather at T = 16384, k = 2, D = 4096
+// (f32, bf16 out) 100 us = 1.02.
 #pragma once
 #include <cstdint>
 
