@@ -839,3 +839,27 @@ def test_layer_second_derivatives_are_refused():
         d.sum().backward()
     with pytest.raises(ValueError, match="token"):
         train.moe_layer_train(x[:0], logits[:0], ups[0], wd, k)
+
+
+def test_layer_with_bf16_logits_and_frozen_inputs():
+    """Gradients in the leaves' own types; tokens or router that take none; an upstream gradient that is one row for all."""
+    T, D, F, E, k = 96, 256, 256, 4, 2
+    x, wr, ups, wd, _ = _layer_inputs(T, D, F, E, False, 15)
+    logits = (x.float() @ wr).bfloat16().requires_grad_()
+    wu, wdn = ups[0].clone().requires_grad_(), wd.clone().requires_grad_()
+    y, routed = train.moe_layer_train(x, logits, wu, wdn, k)
+    (y.sum() + routed.balance_loss).backward()
+    assert logits.grad.dtype == torch.bfloat16 and wu.grad.dtype == torch.bfloat16 and x.grad is None
+    dy = torch.ones((T, D), device=DEV)
+    _, rb, _, rg = _layer_ref(x, logits, ups, wd, routed.ids, torch.ones(T, dtype=torch.bool, device=DEV), dy, False, 1,
+                              T, E, k)
+    assert routed.balance_loss.item() == pytest.approx(rb.item(), rel=1e-5)
+    # _layer_ref's loss has the losses' weights 3 and 2; the experts' gradients do not depend on them.
+    for name, t, r in (("w_up", wu, rg[2]), ("w_down", wdn, rg[3])):
+        assert ((t.grad.double() - r).norm() / r.norm()).item() <= 1e-2, name
+    leaf = x.clone().requires_grad_()
+    y, _ = train.moe_layer_train(leaf, logits.detach(), ups[0], wd, k)
+    y.sum().backward()
+    assert leaf.grad.dtype == torch.bfloat16
+    assert ((leaf.grad.double() - rg[0]).norm() / rg[0].norm()).item() <= 1e-2
+    _lib.device_status(reset=True)
