@@ -279,13 +279,14 @@ __device__ __forceinline__ float lane_max(const Row<V>& v) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// e_i = 2^(l_i log2 e - mxl), mxl = the row maximum times log2 e, rounded: one
-// factor near 1 in all of them, which the ratios p = e / sum(e) and
-// lse = (mxl + log2 sum(e)) ln 2 are free of.  Rows that are not kept have
-// l = -inf throughout, mx = 0 and e = 0.  Where mx log2 e leaves the f32 range
-// (a row masked throughout by the type's lowest value), the maximum is taken
-// off first.
-__device__ __forceinline__ bool far_out(float mx) { return fabsf(mx) > 1e38f; }
+// e_i = 2^(l_i log2 e - mxl), mxl = the row maximum times log2 e, rounded by
+// up to d = 2^-24 |mxl|: a factor 2^d in all of them, which the ratios p = e /
+// sum(e) and lse = (mxl + log2 sum(e)) ln 2 are free of while 2^d is near 1.
+// Rows that are not kept have l = -inf throughout, mx = 0 and e = 0.  Where the
+// maximum is beyond 2^20 (d reaches 0.09 there, and 128 at 1.5e9: every e inf
+// or 0; mx log2 e itself ends at 2.4e38), it is taken off first: a difference
+// of two logits that close has no rounding that matters.
+__device__ __forceinline__ bool far_out(float mx) { return fabsf(mx) > 0x1p20f; }
 template <int V>
 __device__ __forceinline__ float row_exp(const Row<V>& v, float mx, float mxl, Row<V>& e) {
   float2 total = both(0.f);
@@ -708,7 +709,8 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
       w[s] = 0.f;
       if (keep && sel[s] > -INFINITY) {
         // A plain softmax probability is one of the row's e over their sum,
-        // mxl's rounding included (at |mx| = 65504 that is 2e-3).
+        // mxl's rounding included (at |mx| = 65504 that is 2e-3), or formed as
+        // row_exp forms them beyond its range.
         if (!p.sigmoid && !p.normalize && !far_out(mx)) w[s] = ex2_ftz(fmaf(sel[s], kLog2e, -mxl));
         else w[s] = slot_score(sel[s], top, p.sigmoid);
       }
