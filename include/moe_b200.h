@@ -280,7 +280,8 @@ int moe_ep_destroy(moe_ep_t ep);
  *                  their order), inverse (N,) = row of each entry (-1 for an
  *                  id outside [0, E): dropped, status bit 16).  Needs
  *                  moe_permute_workspace_size(N, E) bytes of workspace.
- *                  Rows past sum(group_sizes) of sorted_src are untouched.
+ *                  sorted_src past sum(group_sizes), which dropped entries
+ *                  leave over, is 0: every row of it can be gathered.
  * moe_gather_rows  out[r] = x[sorted_src[r] / k] for rows of row_bytes (a
  *                  multiple of 16) -- X in expert order for moe_fused_mlp.
  * moe_combine_rows y[t] = sum_j topk_weights[t, j] * y_sorted[inverse[t*k+j]]

@@ -1926,7 +1926,8 @@ int moe_route_topk(const float* logits, int64_t T, int32_t E, int32_t k, int32_t
 
 size_t moe_permute_workspace_size(int64_t N, int32_t E) {
   if (N < 0 || E < 1) return 0;
-  return align256((size_t)((N + kPermBlock - 1) / kPermBlock) * (size_t)E * sizeof(int32_t));
+  // Per block and expert an offset; after them the number of routed rows.
+  return align256(((size_t)((N + kPermBlock - 1) / kPermBlock) * (size_t)E + 1) * sizeof(int32_t));
 }
 
 int moe_permute(const int32_t* expert_ids, int64_t N, int32_t E, int32_t* group_sizes, int32_t* sorted_src,

@@ -7,12 +7,14 @@
 //                       full softmax renormalised over the selected experts).
 //   perm_hist_kernel    per block of 512 (token, slot) entries, a histogram
 //                       over experts.
-//   perm_scan_kernel    group sizes, and each block's first row per expert in
-//                       the expert-sorted order.
+//   perm_scan_kernel    group sizes, their sum, and each block's first row per
+//                       expert in the expert-sorted order.
 //   perm_scatter_kernel stable counting sort: entry i = t * k + j lands at
 //                       row inverse[i]; sorted_src[row] = i.  Ranks inside a
 //                       block come from per-warp expert histograms, so the
 //                       order is deterministic (= a stable sort by expert).
+//                       Rows past the last routed one, which dropped entries
+//                       leave over, get entry 0: gather reads every row.
 //   gather_rows_kernel  X_sorted[row] = X[sorted_src[row] / k].
 //   combine_rows_kernel Y[t] = sum_j w[t, j] * Y_sorted[inverse[t * k + j]],
 //                       in slot order (deterministic).
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(1024) perm_scan_kernel(int32_t* __restrict__ b
       if (e0 + lane < E) s_base[e0 + lane] = carry + inc - v;
       carry += __shfl_sync(0xffffffffu, inc, 31);
     }
+    if (lane == 0) block_hist[nblocks * E] = carry;  // rows routed
   }
   __syncthreads();
   for (int e = warp; e < E; e += nw) {
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(kPermBlock) perm_scatter_kernel(const int32_t*
   const int64_t i = (int64_t)blockIdx.x * kPermBlock + threadIdx.x;
   int e = -1;
   if (i < N) {
+    if (i >= __ldg(block_off + (int64_t)gridDim.x * E)) sorted_src[i] = 0;
     e = __ldg(ids + i);
     if (e < 0 || e >= E) e = -1;
   }

@@ -47,15 +47,14 @@ def route_topk(logits: torch.Tensor, k: int):
 def permute(ids: torch.Tensor, num_experts: int, workspace: Optional[torch.Tensor] = None):
     """Stable counting sort of the entries ``i = t * k + j`` of ``ids`` (T, k)
     by expert.  Returns (group_sizes (E,), sorted_src (N,) entry index of each
-    row in expert order, inverse (T, k) row of each entry, -1 if dropped)."""
+    row in expert order - 0 past the last routed row -, inverse (T, k) row of
+    each entry, -1 if dropped)."""
     ids = ids.to(torch.int32).contiguous()
     dev = ids.device
     N = ids.numel()
     L = _lib.lib()
     gs = torch.empty(num_experts, dtype=torch.int32, device=dev)
-    # Rows past sum(group_sizes), which dropped entries leave over, read as
-    # entry 0: gather_rows takes every row of sorted_src.
-    src = torch.zeros(N, dtype=torch.int32, device=dev)
+    src = torch.empty(N, dtype=torch.int32, device=dev)
     inv = torch.empty(ids.shape, dtype=torch.int32, device=dev)
     need = int(L.moe_permute_workspace_size(N, num_experts))
     if workspace is None or workspace.numel() < need:
