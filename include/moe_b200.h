@@ -460,9 +460,11 @@ int moe_route_backward(const void* logits, int32_t elem_type, int64_t ld, int64_
  *
  * moe_combine_rows_backward  y_sorted (rows, D) f32, dy (T, D) of dy_type ->
  *                  dys (rows, D) of dys_type: dys[inverse[t, j]] =
- *                  weights[t, j] dy[t], rows past sum(group_sizes) zero; and
- *                  dw (T, k) f32 = <dy[t], y_sorted[inverse[t, j]]>, 0 where
- *                  dropped.
+ *                  weights[t, j] dy[t], and zero in every row that no entry
+ *                  maps to (past sum(group_sizes), or of an entry that was
+ *                  dropped after moe_permute); dw (T, k) f32 = <dy[t],
+ *                  y_sorted[inverse[t, j]]>, 0 where dropped.  group_sizes is
+ *                  not read: `inverse` alone says which rows are mapped.
  * moe_gather_rows_backward   dxs (rows, D) of dxs_type -> dx (T, D) of
  *                  dx_type: the f32 sum of dxs[inverse[t, j]] in slot order.
  */

@@ -122,8 +122,8 @@ static int route_vec(const void* base, int64_t ld, int E, int type) {
 static int row_threads(int D) { return D >= 1024 ? 256 : D >= 128 ? 32 : 8; }
 
 template <int TPT, int DY, int DYS>
-static int launch_combine(const CombineBwd& p, int zero_blocks, cudaStream_t st) {
-  const unsigned blocks = (unsigned)(p.token_blocks + zero_blocks);
+static int launch_combine(const CombineBwd& p, cudaStream_t st) {
+  const unsigned blocks = (unsigned)((p.T + kRowThreads / TPT - 1) / (kRowThreads / TPT) + p.zero_blocks);
   if (p.k <= 2) combine_bwd_kernel<TPT, DY, DYS, 2><<<blocks, kRowThreads, 0, st>>>(p);
   else if (p.k <= 4) combine_bwd_kernel<TPT, DY, DYS, 4><<<blocks, kRowThreads, 0, st>>>(p);
   else combine_bwd_kernel<TPT, DY, DYS, kRowSlots><<<blocks, kRowThreads, 0, st>>>(p);
@@ -131,19 +131,18 @@ static int launch_combine(const CombineBwd& p, int zero_blocks, cudaStream_t st)
   return 0;
 }
 template <int TPT>
-static int launch_combine_t(CombineBwd p, int dy, int dys, int zero_blocks, cudaStream_t st) {
-  p.token_blocks = (int)((p.T + kRowThreads / TPT - 1) / (kRowThreads / TPT));
+static int launch_combine_t(const CombineBwd& p, int dy, int dys, cudaStream_t st) {
   switch (dy * 3 + dys) {
-    case 0: return launch_combine<TPT, 0, 0>(p, zero_blocks, st);
-    case 1: return launch_combine<TPT, 0, 1>(p, zero_blocks, st);
-    case 2: return launch_combine<TPT, 0, 2>(p, zero_blocks, st);
-    case 3: return launch_combine<TPT, 1, 0>(p, zero_blocks, st);
-    case 4: return launch_combine<TPT, 1, 1>(p, zero_blocks, st);
-    case 5: return launch_combine<TPT, 1, 2>(p, zero_blocks, st);
-    case 6: return launch_combine<TPT, 2, 0>(p, zero_blocks, st);
-    case 7: return launch_combine<TPT, 2, 1>(p, zero_blocks, st);
+    case 0: return launch_combine<TPT, 0, 0>(p, st);
+    case 1: return launch_combine<TPT, 0, 1>(p, st);
+    case 2: return launch_combine<TPT, 0, 2>(p, st);
+    case 3: return launch_combine<TPT, 1, 0>(p, st);
+    case 4: return launch_combine<TPT, 1, 1>(p, st);
+    case 5: return launch_combine<TPT, 1, 2>(p, st);
+    case 6: return launch_combine<TPT, 2, 0>(p, st);
+    case 7: return launch_combine<TPT, 2, 1>(p, st);
   }
-  return launch_combine<TPT, 2, 2>(p, zero_blocks, st);
+  return launch_combine<TPT, 2, 2>(p, st);
 }
 template <int TPT, int DXS, int DX, int VEC>
 static int launch_gather_v(const GatherBwd& p, cudaStream_t st) {
@@ -514,12 +513,23 @@ int moe_combine_rows_backward(const void* dy, int32_t dy_type, const float* y_so
   DevInfo* di;
   if (int r = device_info(&dev, &di)) return r;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  CombineBwd p{dy, y_sorted, inverse, weights, group_sizes, dys, dw, T, rows, k, D, E, 0};
-  const int zero_blocks = (int)std::min<int64_t>(di->sms, (rows * (D / 4) + kRowThreads - 1) / kRowThreads);
+  CombineBwd p{dy, y_sorted, inverse, weights, dys, dw, T, rows, k, D, 0, 0};
+  // Rows that no entry maps to are found by blocks that read all of `inverse`
+  // each, beside the others' work, unless that reads more than zeroing all of
+  // dys beforehand writes (very many short rows).
+  const int64_t row_bytes = (int64_t)D * elem_bytes(dys_type);
+  const int64_t zb = std::max<int64_t>(std::min<int64_t>(kZeroBlocks, (rows * (D / 4) + kRowThreads - 1) / kRowThreads),
+                                       (rows + kZeroRows - 1) / kZeroRows);
+  if (zb * T * k * 4 <= std::max<int64_t>(rows * row_bytes, 8 << 20)) {
+    p.zero_blocks = (int)zb;
+    p.zero_rows = zb ? (int)((rows + zb - 1) / zb) : 0;
+  } else {
+    MOE_CUDA_TRY(cudaMemsetAsync(dys, 0, (size_t)(rows * row_bytes), st));
+  }
   const int tpt = row_threads(D);
-  if (tpt == 256) return launch_combine_t<256>(p, dy_type, dys_type, zero_blocks, st);
-  if (tpt == 32) return launch_combine_t<32>(p, dy_type, dys_type, zero_blocks, st);
-  return launch_combine_t<8>(p, dy_type, dys_type, zero_blocks, st);
+  if (tpt == 256) return launch_combine_t<256>(p, dy_type, dys_type, st);
+  if (tpt == 32) return launch_combine_t<32>(p, dy_type, dys_type, st);
+  return launch_combine_t<8>(p, dy_type, dys_type, st);
 }
 
 int moe_gather_rows_backward(const void* dxs, int32_t dxs_type, const int32_t* inverse, int64_t T, int32_t k,

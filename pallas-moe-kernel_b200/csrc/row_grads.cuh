@@ -45,13 +45,63 @@ struct CombineBwd {
   const float* y_sorted;    // (rows, D)
   const int32_t* inverse;   // (T, k)
   const float* weights;     // (T, k)
-  const int32_t* group_sizes;  // (E,)
   void* dys;                // (rows, D)
   float* dw;                // (T, k)
   int64_t T, rows;
-  int32_t k, D, E;
-  int32_t token_blocks;     // blocks past these zero the rows behind sum(group_sizes)
+  int32_t k, D;
+  int32_t zero_blocks;      // the first blocks: zero the rows that no entry maps to, zero_rows each
+  int32_t zero_rows;
 };
+
+constexpr int kZeroRows = 32768;  // most rows of a zeroing block: a bit each in shared memory (4 KB)
+constexpr int kZeroBlocks = 32;   // zeroing blocks where those are enough
+
+// Rows [lo, lo + p.zero_rows) of dys that no entry maps to (behind the last
+// routed row, or dropped after the permutation): zero.  The block looks through
+// all of `inverse` and marks what falls into its rows, beside the tokens'
+// blocks.  At T = 32768, k = 16 (2 MB of entries, about 30 us a block) one such
+// block per SM took L2's bandwidth from the others (D = 128, bf16 out: 94 -> 122
+// us); with 32 of them it is 100, and at T = 8192, k = 8, D = 7168 461 as without.
+// A call, not inlined: with it in the kernel the tokens' loop got 30 registers
+// less and ran 15% longer.
+template <int DYS>
+__device__ __noinline__ void zero_unmapped(const CombineBwd& p, uint32_t* s_map) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t lo = (int64_t)blockIdx.x * p.zero_rows, n = p.T * p.k;
+  const int rows = (int)max((int64_t)0, min((int64_t)p.zero_rows, p.rows - lo));
+  const int words = (rows + 31) / 32;
+  for (int w = threadIdx.x; w < words; w += kRowThreads) s_map[w] = 0;
+  __syncthreads();
+  const auto mark = [&](int r) {  // rows end below 2^31: a negative r is past them all
+    const uint32_t at = (uint32_t)r - (uint32_t)lo;
+    if (at < (uint32_t)rows) atomicOr(s_map + (at >> 5), 1u << (at & 31));
+  };
+  // Entries in fours from the first 16-byte boundary on, eight fours in flight.
+  const int64_t head = min(n, (int64_t)((0 - (reinterpret_cast<uintptr_t>(p.inverse) >> 2)) & 3));
+  const int64_t fours = (n - head) / 4, tail = head + 4 * fours;
+  if (threadIdx.x < head) mark(__ldg(p.inverse + threadIdx.x));
+  if (threadIdx.x < n - tail) mark(__ldg(p.inverse + tail + threadIdx.x));
+  const int4* body = reinterpret_cast<const int4*>(p.inverse + head);
+  constexpr int kAhead = 8;
+  for (int64_t i0 = threadIdx.x; i0 < fours; i0 += kAhead * kRowThreads) {
+    int4 r[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      r[u] = i0 + u * kRowThreads < fours ? __ldg(body + i0 + u * kRowThreads) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) mark(r[u].x), mark(r[u].y), mark(r[u].z), mark(r[u].w);
+  }
+  __syncthreads();
+  const int n4 = p.D >> 2;
+  for (int w = warp; w < words; w += kRowThreads / 32) {
+    uint32_t left = ~s_map[w];
+    if (32 * w + 32 > rows) left &= (1u << (rows & 31)) - 1u;
+    for (; left; left &= left - 1) {
+      const int64_t row = (lo + 32 * w + __ffs(left) - 1) * n4;
+      for (int c = lane; c < n4; c += 32) row_store4<DYS>(p.dys, row + c, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+  }
+}
 
 // The sum over a token's TPT threads, valid in the first of them.
 template <int TPT>
@@ -71,32 +121,17 @@ __device__ __forceinline__ float token_sum(float v, float* s_w) {
 }
 
 template <int TPT, int DY, int DYS, int SLOTS>
-__global__ void __launch_bounds__(kRowThreads) combine_bwd_kernel(const CombineBwd p) {
+__global__ void __launch_bounds__(kRowThreads) combine_bwd_kernel(const __grid_constant__ CombineBwd p) {
   constexpr int U = kRowSlots / SLOTS;
   __shared__ float s_w[kRowThreads / 32];
+  __shared__ uint32_t s_map[kZeroRows / 32];
   const int n4 = p.D >> 2;
-  if (blockIdx.x >= p.token_blocks) {
-    // Rows behind the last routed one take no part: zero.
-    __shared__ int s_total;
-    if (threadIdx.x < 32) {
-      int64_t sum = 0;
-      for (int e = threadIdx.x; e < p.E; e += 32) {
-        const int g = __ldg(p.group_sizes + e);
-        sum += g > 0 ? g : 0;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (threadIdx.x == 0) s_total = (int)(sum < p.rows ? sum : p.rows);
-    }
-    __syncthreads();
-    const int zb = gridDim.x - p.token_blocks;
-    for (int64_t i = (int64_t)s_total * n4 + (blockIdx.x - p.token_blocks) * kRowThreads + threadIdx.x; i < p.rows * n4;
-         i += (int64_t)zb * kRowThreads)
-      row_store4<DYS>(p.dys, i, make_float4(0.f, 0.f, 0.f, 0.f));
+  if (blockIdx.x < p.zero_blocks) {
+    zero_unmapped<DYS>(p, s_map);
     return;
   }
   const int k = p.k, me = threadIdx.x % TPT;
-  const int64_t t = (int64_t)blockIdx.x * (kRowThreads / TPT) + threadIdx.x / TPT;
+  const int64_t t = (int64_t)(blockIdx.x - p.zero_blocks) * (kRowThreads / TPT) + threadIdx.x / TPT;
   const bool inside = t < p.T;
   for (int j0 = 0; j0 < k; j0 += SLOTS) {
     int64_t row[SLOTS];

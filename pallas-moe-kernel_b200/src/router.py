@@ -162,9 +162,11 @@ def combine_rows_backward(dy: torch.Tensor, y_sorted: torch.Tensor, inverse: tor
                           ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Backward of :func:`combine_rows` for the upstream gradient ``dy``
     (T, D): (dys, dw) with ``dys[inverse[t, j]] = weights[t, j] * dy[t]`` in
-    ``dtype`` - rows past ``sum(group_sizes)`` zero - and the f32 weights'
-    gradient ``dw[t, j] = <dy[t], y_sorted[inverse[t, j]]>``, 0 at dropped
-    entries.  bfloat16 ``dys`` are what the experts' backward multiplies."""
+    ``dtype`` - zero in every row that no entry maps to, past
+    ``sum(group_sizes)`` or of entries dropped after :func:`permute` - and the
+    f32 weights' gradient ``dw[t, j] = <dy[t], y_sorted[inverse[t, j]]>``, 0 at
+    dropped entries.  bfloat16 ``dys`` are what the experts' backward
+    multiplies."""
     return _lib.native().combine_backward(dy, y_sorted, inverse, weights, group_sizes, _out_elem(dtype))
 
 
