@@ -518,11 +518,12 @@ int moe_combine_rows_backward(const void* dy, int32_t dy_type, const float* y_so
   // each, beside the others' work, unless that reads more than zeroing all of
   // dys beforehand writes (very many short rows).
   const int64_t row_bytes = (int64_t)D * elem_bytes(dys_type);
-  const int64_t zb = std::max<int64_t>(std::min<int64_t>(kZeroBlocks, (rows * (D / 4) + kRowThreads - 1) / kRowThreads),
-                                       (rows + kZeroRows - 1) / kZeroRows);
-  if (zb * T * k * 4 <= std::max<int64_t>(rows * row_bytes, 8 << 20)) {
-    p.zero_blocks = (int)zb;
-    p.zero_rows = zb ? (int)((rows + zb - 1) / zb) : 0;
+  int shift = 0;
+  while (shift < zero_shift_most(D) && ((int64_t)kRowThreads << shift) < rows * (D / 4)) ++shift;
+  while (((int64_t)kZeroRows << shift) < rows) ++shift;
+  if (((T * k * 4) << shift) <= std::max<int64_t>(rows * row_bytes, 8 << 20)) {
+    p.zero_blocks = rows ? 1 << shift : 0;
+    p.zero_shift = shift;
   } else {
     MOE_CUDA_TRY(cudaMemsetAsync(dys, 0, (size_t)(rows * row_bytes), st));
   }

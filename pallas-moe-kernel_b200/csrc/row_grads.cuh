@@ -49,32 +49,38 @@ struct CombineBwd {
   float* dw;                // (T, k)
   int64_t T, rows;
   int32_t k, D;
-  int32_t zero_blocks;      // the first blocks: zero the rows that no entry maps to, zero_rows each
-  int32_t zero_rows;
+  int32_t zero_blocks;      // the first blocks, 0 or 2^zero_shift: zero the rows that no entry maps to
+  int32_t zero_shift;
 };
 
 constexpr int kZeroRows = 32768;  // most rows of a zeroing block: a bit each in shared memory (4 KB)
-constexpr int kZeroBlocks = 32;   // zeroing blocks where those are enough
 
-// Rows [lo, lo + p.zero_rows) of dys that no entry maps to (behind the last
-// routed row, or dropped after the permutation): zero.  The block looks through
-// all of `inverse` and marks what falls into its rows, beside the tokens'
-// blocks.  At T = 32768, k = 16 (2 MB of entries, about 30 us a block) one such
-// block per SM took L2's bandwidth from the others (D = 128, bf16 out: 94 -> 122
-// us); with 32 of them it is 100, and at T = 8192, k = 8, D = 7168 461 as without.
-// A call, not inlined: with it in the kernel the tokens' loop got 30 registers
-// less and ran 15% longer.
+// Zeroing blocks where kZeroRows allows as few: 2^this.  Each reads all of
+// `inverse`, so fewer for short rows (T = 32768, k = 16: D = 128 to bf16 94 us
+// without any, 101 with 32, 108 with 64, 122 with one per SM; D = 256 to f32 185,
+// 193, 199, 262); long rows need more for their stores (T = 4096, k = 8, D = 512,
+// nine tokens in ten dropped: 45 us with 32, 29 with 64; T = 8192, D = 7168 481
+// and 318, with none dropped 461 like without).
+constexpr int zero_shift_most(int D) { return D >= 512 ? 6 : 5; }
+
+// The rows of dys that no entry maps to (behind the last routed row, or dropped
+// after the permutation): zero.  A zeroing block looks through all of `inverse`
+// and marks what falls into its rows, beside the tokens' blocks; blocks take 32
+// rows in turn, so that a tail of padding is shared.  A call, not inlined: with
+// it in the kernel the tokens' loop got 30 registers less and ran 15% longer.
 template <int DYS>
 __device__ __noinline__ void zero_unmapped(const CombineBwd& p, uint32_t* s_map) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t lo = (int64_t)blockIdx.x * p.zero_rows, n = p.T * p.k;
-  const int rows = (int)max((int64_t)0, min((int64_t)p.zero_rows, p.rows - lo));
-  const int words = (rows + 31) / 32;
-  for (int w = threadIdx.x; w < words; w += kRowThreads) s_map[w] = 0;
+  const int shift = p.zero_shift;
+  const int64_t n = p.T * p.k;
+  const uint32_t me = blockIdx.x, all = (uint32_t)((p.rows + 31) >> 5);          // words of 32 rows
+  const uint32_t words = all > me ? (all - me - 1 >> shift) + 1 : 0;             // this block's: me, me + 2^shift, ...
+  for (uint32_t w = threadIdx.x; w < words; w += kRowThreads) s_map[w] = 0;
   __syncthreads();
-  const auto mark = [&](int r) {  // rows end below 2^31: a negative r is past them all
-    const uint32_t at = (uint32_t)r - (uint32_t)lo;
-    if (at < (uint32_t)rows) atomicOr(s_map + (at >> 5), 1u << (at & 31));
+  const auto mark = [&](int r) {
+    const uint32_t w = (uint32_t)r >> 5;
+    if ((w & ((1u << shift) - 1u)) == me && (uint32_t)r < (uint32_t)p.rows)
+      atomicOr(s_map + (w >> shift), 1u << (r & 31));
   };
   // Entries in fours from the first 16-byte boundary on, eight fours in flight.
   const int64_t head = min(n, (int64_t)((0 - (reinterpret_cast<uintptr_t>(p.inverse) >> 2)) & 3));
@@ -92,13 +98,21 @@ __device__ __noinline__ void zero_unmapped(const CombineBwd& p, uint32_t* s_map)
     for (int u = 0; u < kAhead; ++u) mark(r[u].x), mark(r[u].y), mark(r[u].z), mark(r[u].w);
   }
   __syncthreads();
-  const int n4 = p.D >> 2;
-  for (int w = warp; w < words; w += kRowThreads / 32) {
+  // Stores of 16 bytes where a row is made of them, else of 8 (the 16-bit types).
+  const int64_t row_bytes = (int64_t)p.D * (DYS == kElemF32 ? 4 : 2);
+  const bool wide = ((row_bytes | reinterpret_cast<intptr_t>(p.dys)) & 15) == 0;
+  for (uint32_t w = warp; w < words; w += kRowThreads / 32) {
     uint32_t left = ~s_map[w];
-    if (32 * w + 32 > rows) left &= (1u << (rows & 31)) - 1u;
+    const int64_t row0 = (int64_t)((w << shift) + me) * 32;
+    if (row0 + 32 > p.rows) left &= (1u << (p.rows & 31)) - 1u;
     for (; left; left &= left - 1) {
-      const int64_t row = (lo + 32 * w + __ffs(left) - 1) * n4;
-      for (int c = lane; c < n4; c += 32) row_store4<DYS>(p.dys, row + c, make_float4(0.f, 0.f, 0.f, 0.f));
+      uint8_t* row = static_cast<uint8_t*>(p.dys) + (row0 + __ffs(left) - 1) * row_bytes;
+      if (wide) {
+#pragma unroll 4
+        for (int c = lane; c < (int)(row_bytes >> 4); c += 32) reinterpret_cast<uint4*>(row)[c] = make_uint4(0, 0, 0, 0);
+      } else {
+        for (int c = lane; c < (int)(row_bytes >> 3); c += 32) reinterpret_cast<uint2*>(row)[c] = make_uint2(0, 0);
+      }
     }
   }
 }

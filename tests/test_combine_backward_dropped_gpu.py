@@ -50,7 +50,7 @@ def test_rows_without_an_entry_are_zero(T, k, D, E, drop, extra, out_t):
     assert torch.all(dw[inv < 0] == 0)
 
 
-@pytest.mark.parametrize("T,k,D", [(300_000, 2, 8), (100_001, 2, 1024), (40_000, 16, 32), (8192, 8, 256)])
+@pytest.mark.parametrize("T,k,D", [(1_100_001, 2, 512), (300_000, 2, 8), (100_001, 2, 1024), (40_000, 16, 32), (8192, 8, 256)])
 def test_many_rows(T, k, D):
     """Rows in a random order, a tenth of the entries dropped, bits for bits (weights are powers of two)."""
     g = torch.Generator(device=DEV)
