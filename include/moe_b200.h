@@ -489,7 +489,10 @@ int moe_gather_rows_backward(const void* dxs, int32_t dxs_type, const int32_t* i
  *                  here.  norm (device f32, or NULL with a given norm)
  *                  receives the norm.  `out` may be `in` (same type and
  *                  strides), and then nothing is written when the factor is
- *                  1; otherwise an `out` overlaps no tensor of the list.  A
+ *                  1; otherwise an `out` has no byte in common with a tensor
+ *                  of the list, nor with another `out`, nor either norm with
+ *                  an `out` (refused: MOE_ERR_INVALID_ARG; slices of one
+ *                  matrix that interleave have none).  A
  *                  NaN norm makes every output NaN, an infinite one 0 (NaN
  *                  where the element is infinite).
  * Workspace: moe_grad_norm_workspace_size(n) bytes, 256-byte aligned.

@@ -3,7 +3,9 @@
 // movement, and gradient norms and clipping.  Declarations:
 // include/moe_b200.h.
 #include <algorithm>
+#include <cstdint>
 #include <cstdlib>
+#include <utility>
 
 #include "abi_util.h"
 #include "grad_norm.cuh"
@@ -210,38 +212,120 @@ static int check_tensors(const moe_tensor_desc* t, int n, int norm_type, bool wi
   return 0;
 }
 
-// Outputs that share memory would be scaled twice, in an order nobody knows.
-// Dense tensors are compared by their ranges, those of several rows by their
-// first element (rows of two slices of one matrix interleave).  Lists come in
-// the order of their addresses more often than not: that needs no sorting.
+// Bytes of a tensor: `rows` runs of `bytes`, `ld` apart.
+struct Span {
+  uintptr_t lo;
+  uint64_t rows, bytes, ld;
+  uintptr_t end() const { return lo + (rows - 1) * ld + bytes; }
+};
+static Span in_span(const moe_tensor_desc& d) {
+  const uint64_t eb = elem_bytes(d.in_type);
+  return {reinterpret_cast<uintptr_t>(d.in), (uint64_t)d.rows, d.cols * eb, d.rows > 1 ? d.in_ld * eb : 0};
+}
+static Span out_span(const moe_tensor_desc& d) {
+  const uint64_t eb = elem_bytes(d.out_type);
+  return {reinterpret_cast<uintptr_t>(d.out), (uint64_t)d.rows, d.cols * eb, d.rows > 1 ? d.out_ld * eb : 0};
+}
+
+// Whether two tensors have a byte in common: slices of one matrix interleave
+// without.
+static bool spans_meet(Span a, Span b) {
+  if (a.lo >= b.end() || b.lo >= a.end()) return false;
+  if (a.rows > 1 && b.rows > 1 && a.ld == b.ld) {
+    // Row j of b starts at byte `off` of a's row `first` + j, and may run into the next.
+    if (a.lo > b.lo) std::swap(a, b);
+    const uint64_t first = (b.lo - a.lo) / a.ld, off = (b.lo - a.lo) % a.ld;
+    return (off < a.bytes && first < a.rows) || (off + b.bytes > a.ld && first + 1 < a.rows);
+  }
+  if (a.rows > b.rows) std::swap(a, b);
+  for (uint64_t r = 0; r < a.rows; ++r) {
+    const uintptr_t lo = a.lo + r * a.ld, hi = lo + a.bytes;
+    // The first row of b that ends past lo.
+    const uint64_t j = b.rows == 1 || lo < b.lo + b.bytes ? 0 : (lo - b.lo - b.bytes) / b.ld + 1;
+    if (j < b.rows && b.lo + j * b.ld < hi && b.lo + j * b.ld + b.bytes > lo) return true;
+  }
+  return false;
+}
+
+// Outputs that share memory would be scaled twice, and a gradient that shares
+// it with another's output read before or after that: neither has an order.
+// Lists come in the order of their addresses more often than not: that needs
+// no sorting.
 static int check_outputs(const moe_tensor_desc* t, int n) {
-  auto start = [&](int i) { return reinterpret_cast<uintptr_t>(t[i].out); };
-  auto end = [&](int i) { return start(i) + (t[i].rows == 1 ? t[i].cols : 1) * elem_bytes(t[i].out_type); };
   auto live = [&](int i) { return t[i].rows && t[i].cols; };
-  int last = -1;
-  bool sorted = true, apart = true;
-  for (int i = 0; i < n; ++i)
-    if (live(i) && t[i].out == t[i].in && (t[i].in_type != t[i].out_type || (t[i].rows > 1 && t[i].in_ld != t[i].out_ld)))
-      return fail(MOE_ERR_INVALID_ARG, "tensor %d is scaled in place with another type or stride", i);
+  uintptr_t last = 0, out_lo = UINTPTR_MAX, out_hi = 0, in_lo = UINTPTR_MAX, in_hi = 0;
+  bool sorted = true;
   for (int i = 0; i < n; ++i) {
     if (!live(i)) continue;
-    if (last >= 0 && start(i) < end(last)) {
-      sorted = false;
-      break;
+    const bool in_place = t[i].out == t[i].in;
+    if (in_place && (t[i].in_type != t[i].out_type || (t[i].rows > 1 && t[i].in_ld != t[i].out_ld)))
+      return fail(MOE_ERR_INVALID_ARG, "tensor %d is scaled in place with another type or stride", i);
+    const Span o = out_span(t[i]);
+    sorted = sorted && o.lo >= last;
+    last = o.end();
+    out_lo = std::min(out_lo, o.lo);
+    out_hi = std::max(out_hi, o.end());
+    if (!in_place) {
+      const Span g = in_span(t[i]);
+      in_lo = std::min(in_lo, g.lo);
+      in_hi = std::max(in_hi, g.end());
     }
-    last = i;
   }
-  if (!sorted) {
-    int* order = static_cast<int*>(malloc(sizeof(int) * (size_t)n));
-    if (!order) return fail(MOE_ERR_INVALID_ARG, "no memory for a list of %d tensors", n);
-    int m = 0;
-    for (int i = 0; i < n; ++i)
-      if (live(i)) order[m++] = i;
-    std::sort(order, order + m, [&](int a, int b) { return start(a) < start(b); });
-    for (int i = 1; i < m; ++i) apart = apart && start(order[i]) >= end(order[i - 1]);
-    free(order);
+  if (sorted && (in_lo >= out_hi || out_lo >= in_hi)) return 0;
+  struct Item {
+    Span s;
+    uintptr_t end;
+    int tensor;
+    bool out;
+  };
+  // All of them by first byte; those that still run when one starts are compared with it.
+  Item* items = static_cast<Item*>(malloc(sizeof(Item) * 2 * (size_t)n));
+  int* open = static_cast<int*>(malloc(sizeof(int) * 2 * (size_t)n));
+  int m = 0, first = -1, second = -1;
+  if (items && open) {
+    for (int i = 0; i < n; ++i) {
+      if (!live(i)) continue;
+      const Span o = out_span(t[i]), g = in_span(t[i]);
+      items[m++] = Item{o, o.end(), i, true};
+      if (t[i].out != t[i].in) items[m++] = Item{g, g.end(), i, false};
+    }
+    std::sort(items, items + m, [](const Item& x, const Item& y) { return x.s.lo < y.s.lo; });
+    int opened = 0;
+    for (int x = 0; x < m && first < 0; ++x) {
+      int kept = 0;
+      for (int y = 0; y < opened; ++y) {
+        const Item& o = items[open[y]];
+        if (o.end <= items[x].s.lo) continue;
+        open[kept++] = open[y];
+        if ((o.out || items[x].out) && spans_meet(o.s, items[x].s)) first = open[y], second = x;
+      }
+      opened = kept;
+      open[opened++] = x;
+    }
   }
-  return apart ? 0 : fail(MOE_ERR_INVALID_ARG, "an output is in the list twice, or two of them share memory");
+  const bool memory = items && open, outs = first >= 0 && items[first].out && items[second].out;
+  const int a = first >= 0 ? items[first].tensor : -1, b = first >= 0 ? items[second].tensor : -1;
+  free(items);
+  free(open);
+  if (!memory) return fail(MOE_ERR_INVALID_ARG, "no memory for a list of %d tensors", n);
+  if (first < 0) return 0;
+  if (outs)
+    return fail(MOE_ERR_INVALID_ARG, "an output is in the list twice, or two of them share memory: tensors %d and %d",
+                a, b);
+  return fail(MOE_ERR_INVALID_ARG, "an output shares memory with a gradient: tensors %d and %d", a, b);
+}
+
+// A norm inside the list would be scaled, or written while the list is read.
+static int check_norm_place(const moe_tensor_desc* t, int n, const float* given, const float* norm) {
+  const Span g{reinterpret_cast<uintptr_t>(given), 1, given ? sizeof(float) : 0, 0};
+  const Span w{reinterpret_cast<uintptr_t>(norm), 1, norm && norm != given ? sizeof(float) : 0, 0};
+  for (int i = 0; i < n; ++i) {
+    if (!t[i].rows || !t[i].cols) continue;
+    const Span o = out_span(t[i]);
+    if ((g.bytes && spans_meet(g, o)) || (w.bytes && (spans_meet(w, o) || spans_meet(w, in_span(t[i])))))
+      return fail(MOE_ERR_INVALID_ARG, "the norm lies in tensor %d", i);
+  }
+  return 0;
 }
 
 static int entry_head(const GradEntry& e) {
@@ -593,6 +677,7 @@ int moe_clip_grads(const moe_tensor_desc* tensors, int32_t n, int32_t norm_type,
   if (!given_norm && !norm) return fail(MOE_ERR_INVALID_ARG, "null norm");
   if (!given_norm)
     if (int r = check_norm_space(n, workspace, workspace_bytes)) return r;
+  if (int r = check_norm_place(tensors, n, given_norm, norm)) return r;
   int dev;
   DevInfo* di;
   if (int r = device_info(&dev, &di)) return r;

@@ -54,10 +54,11 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, norm_type: fl
     the norm they had (see :func:`grad_norm`).
 
     In place, or into ``out``: tensors of the same shapes, of any of the three
-    types (one rounding from the f32 product), that share no memory with the
-    gradients.  In place nothing is written where the factor is 1.  A NaN norm
-    makes every result NaN, as the product says; check the returned norm to
-    skip such a step."""
+    types (one rounding from the f32 product).  An output that shares memory
+    with another output or with a gradient is refused (slices of one matrix
+    that interleave are not).  In place nothing is written where the factor is
+    1.  A NaN norm makes every result NaN, as the product says; check the
+    returned norm to skip such a step."""
     return _lib.native().clip(grads, max_norm, _norm_code(norm_type), None, out)
 
 
