@@ -399,6 +399,14 @@ List describe(PyObject* grads, PyObject* out) {
   l.keep.insert(l.keep.end(), outs.begin(), outs.end());
   return l;
 }
+// Tells autograd that a call wrote the outputs (the gradients, in place): a
+// graph that saved one of them raises at its backward, as after any in-place
+// operation.
+void written(const List& l) {
+  const size_t n = l.d.size();
+  for (size_t i = l.keep.size() > n ? n : 0; i < l.keep.size(); ++i)
+    if (!l.keep[i].is_inference()) l.keep[i].unsafeGetTensorImpl()->bump_version();
+}
 at::Tensor no_gradients() { return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA)); }
 
 // (gradients, norm type)
@@ -437,6 +445,7 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       "total_norm must be a float32 scalar tensor on the gradients' device");
     check(p_clip(l.d.data(), (int32_t)l.d.size(), (int32_t)integer(a[2]), max_norm, given->data_ptr<float>(), nullptr,
                  nullptr, 0, stream));
+    written(l);
     return THPVariable_Wrap(*given);
   }
   at::Tensor norm = empty({}, at::kFloat, *l.dev);
@@ -444,6 +453,7 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor ws = workspace(*l.dev, stream, need, capturing());
   check(p_clip(l.d.data(), (int32_t)l.d.size(), (int32_t)integer(a[2]), max_norm, nullptr, norm.data_ptr<float>(),
                ws.data_ptr(), need, stream));
+  written(l);
   return THPVariable_Wrap(norm);
   END_HANDLE_TH_ERRORS
 }
