@@ -814,6 +814,9 @@ struct RouteBackward {
 //   normalised                   w_j (dw_j - <dw, w>) (times 1 - s_j, sigmoid)
 //   plain softmax probability    w_j dw_j, and -p_e <dw, w> on every expert
 //   plain sigmoid                w_j dw_j (1 - s_j)
+// Normalised weights sum to 1 but for their rounding, which times what all dw of
+// a row share would stay over where the formula cancels; the first slot's dw is
+// taken off all of them before (one weight alone gets exactly 0).
 // It is formed in the slots' lanes and added to the row in shared memory, on
 // its way to the store (a register exchange takes k V compares a lane).
 // WEIGHTS: there is such a part (the losses alone spare its registers).
@@ -895,6 +898,12 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
           id[s] = -1;
           w[s] = g[s] = 0.f;
         }
+      }
+      float first = __shfl_sync(0xffffffffu, g[0], lane / G * G);
+      if (!p.normalize) first = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if (id[s] >= 0) g[s] -= first;
         dot = fmaf(w[s], g[s], dot);
         // 1 - sigmoid of the slot's logit, into its weight: w is done with.
         if (p.sigmoid && id[s] >= 0)
