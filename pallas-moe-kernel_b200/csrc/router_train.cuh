@@ -828,172 +828,204 @@ __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gl = lane % G;
   const int e0 = gl * V, E = p.E, k = p.k;
-  const int64_t seq = blockIdx.x / p.chunks;
-  const int chunk = blockIdx.x % p.chunks;
-  const int64_t per = route_share(p.seq_len, p.chunks, kRouteWarps * TPW);
-  const int64_t lo = seq * p.seq_len + chunk * per;
-  const int64_t hi = seq * p.seq_len + min(p.seq_len, (chunk + 1) * per);
   float4* fours = s_rows[warp];
-  {  // the first rows come while the experts' factors are made
-    const int64_t t = lo + warp * TPW + lane / G;
-    row_prefetch<V>(p.logits, p.type, t * p.ld, e0, E, t < hi);
-  }
 
-  // Tokens in all sequences and sequences with any.
-  const int ns = __ldg(p.tokens + seq);
-  int all = ns, live_seqs = ns > 0;
-  if (p.S > 1) {
-    all = live_seqs = 0;
-    for (int i = lane; i < p.S; i += 32) {
+  // Tokens in all sequences and sequences with any: by each warp where that is
+  // one load a lane, else by the block, to wait in shared memory.  So does the
+  // run of tokens in work: registers are what the rows need.
+  __shared__ int s_all, s_live;
+  __shared__ uint32_t s_unit;
+  if (threadIdx.x == 0) s_unit = blockIdx.x;
+  if (p.S > 32) {
+    __shared__ int s_n[2][kRouteWarps];
+    int all = 0, live_seqs = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.S; i += kRouteThreads) {
       const int m = __ldg(p.tokens + i);
       all += m;
       live_seqs += m > 0;
     }
     all = __reduce_add_sync(0xffffffffu, all);
     live_seqs = __reduce_add_sync(0xffffffffu, live_seqs);
+    if (lane == 0) s_n[0][warp] = all, s_n[1][warp] = live_seqs;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      all = live_seqs = 0;
+      for (int w = 0; w < kRouteWarps; ++w) all += s_n[0][w], live_seqs += s_n[1][w];
+      s_all = all, s_live = live_seqs;
+    }
+    __syncthreads();
   }
-  // dB / (S' N) (1 / (k N)) (c E - k N): the integer part is exact (in 32 bits
-  // where k N E, which bounds c E, fits).
-  const float db = p.d_balance && ns > 0 ? __ldg(p.d_balance) / ((float)live_seqs * (float)ns) : 0.f;
-  const float dz = p.d_z && all > 0 ? 2.f * __ldg(p.d_z) / (float)all : 0.f;
-  // They lie in shared memory, a lane's experts in fours: the registers that
-  // they would take hold more rows instead.
-  __shared__ float4 s_f[V / 4][32];
-  const float kn = db / (float)((int64_t)k * (ns > 0 ? ns : 1));
-  const bool narrow = (int64_t)k * ns * E < (int64_t)1 << 31;
-  for (int i = threadIdx.x; i < 32 * V; i += kRouteThreads) {
-    const int l = i / V, x = i % V, e = l % G * V + x;
-    const int c = e < E ? __ldg(p.counts + seq * E + e) : 0;
-    const float over = narrow ? (float)(c * E - k * ns) : (float)((int64_t)c * E - (int64_t)k * ns);
-    reinterpret_cast<float*>(&s_f[x / 4][l])[x % 4] = e < E ? over * kn : 0.f;
-  }
-  __syncthreads();
-  const auto f = [&](int i) {  // pair i of the lane's experts
-    return reinterpret_cast<const float2*>(&s_f[i / 2][lane])[i % 2];
-  };
 
-  for (int64_t base = lo + warp * TPW; base < hi; base += kRouteWarps * TPW) {
-    const int64_t t = base + lane / G;
-    const bool inside = t < hi;
-    const bool live = inside && (!p.mask || __ldg(p.mask + t));
-    Row<V> v;
-    row_load(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
-    const int64_t next = t + kRouteWarps * TPW;
-    row_prefetch<V>(p.logits, p.type, next * p.ld, e0, E, next < hi);
-    // The weights' part per slot.
-    int id[KS];
-    float g[KS], w[KS], dot = 0.f;
-    if constexpr (WEIGHTS) {
+  // A block's runs of tokens: one, or with very many sequences several.
+  for (uint32_t unit = blockIdx.x;;) {
+    const int64_t seq = unit / p.chunks;
+    const int chunk = unit % p.chunks;
+    const int64_t per = route_share(p.seq_len, p.chunks, kRouteWarps * TPW);
+    const int64_t lo = seq * p.seq_len + chunk * per;
+    const int64_t hi = seq * p.seq_len + min(p.seq_len, (chunk + 1) * per);
+    {  // the first rows come while the experts' factors are made
+      const int64_t t = lo + warp * TPW + lane / G;
+      row_prefetch<V>(p.logits, p.type, t * p.ld, e0, E, t < hi);
+    }
+    const int ns = __ldg(p.tokens + seq);
+    int all = ns, live_seqs = ns > 0;
+    if (p.S > 32) {
+      all = s_all, live_seqs = s_live;
+    } else if (p.S > 1) {
+      const int m = lane < p.S ? __ldg(p.tokens + lane) : 0;
+      all = __reduce_add_sync(0xffffffffu, m);
+      live_seqs = __reduce_add_sync(0xffffffffu, (int)(m > 0));
+    }
+    // dB / (S' N) (1 / (k N)) (c E - k N): the integer part is exact (in 32 bits
+    // where k N E, which bounds c E, fits).
+    const float db = p.d_balance && ns > 0 ? __ldg(p.d_balance) / ((float)live_seqs * (float)ns) : 0.f;
+    const float dz = p.d_z && all > 0 ? 2.f * __ldg(p.d_z) / (float)all : 0.f;
+    // They lie in shared memory, a lane's experts in fours: the registers that
+    // they would take hold more rows instead.
+    __shared__ float4 s_f[V / 4][32];
+    const float kn = db / (float)((int64_t)k * (ns > 0 ? ns : 1));
+    const bool narrow = (int64_t)k * ns * E < (int64_t)1 << 31;
+    for (int i = threadIdx.x; i < 32 * V; i += kRouteThreads) {
+      const int l = i / V, x = i % V, e = l % G * V + x;
+      const int c = e < E ? __ldg(p.counts + seq * E + e) : 0;
+      const float over = narrow ? (float)(c * E - k * ns) : (float)((int64_t)c * E - (int64_t)k * ns);
+      reinterpret_cast<float*>(&s_f[x / 4][l])[x % 4] = e < E ? over * kn : 0.f;
+    }
+    __syncthreads();
+    const auto f = [&](int i) {  // pair i of the lane's experts
+      return reinterpret_cast<const float2*>(&s_f[i / 2][lane])[i % 2];
+    };
+
+    for (int64_t base = lo + warp * TPW; base < hi; base += kRouteWarps * TPW) {
+      const int64_t t = base + lane / G;
+      const bool inside = t < hi;
+      const bool live = inside && (!p.mask || __ldg(p.mask + t));
+      Row<V> v;
+      row_load(p.logits, p.type, p.vec, t * p.ld, e0, E, live, v);
+      const int64_t next = t + kRouteWarps * TPW;
+      row_prefetch<V>(p.logits, p.type, next * p.ld, e0, E, next < hi);
+      // The weights' part per slot.
+      int id[KS];
+      float g[KS], w[KS], dot = 0.f;
+      if constexpr (WEIGHTS) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int j = s * G + gl;
-        const bool on = live && j < k;  // the three loads do not wait for one another
-        id[s] = on ? __ldg(p.ids + t * k + j) : -1;
-        w[s] = on ? __ldg(p.weights + t * k + j) : 0.f;
-        g[s] = on ? __ldg(p.d_weights + t * k + j) : 0.f;
-      }
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        if (id[s] < 0 || id[s] >= E) {  // dropped, whatever its gradient holds
-          id[s] = -1;
-          w[s] = g[s] = 0.f;
+        for (int s = 0; s < KS; ++s) {
+          const int j = s * G + gl;
+          const bool on = live && j < k;  // the three loads do not wait for one another
+          id[s] = on ? __ldg(p.ids + t * k + j) : -1;
+          w[s] = on ? __ldg(p.weights + t * k + j) : 0.f;
+          g[s] = on ? __ldg(p.d_weights + t * k + j) : 0.f;
         }
-      }
-      float first = __shfl_sync(0xffffffffu, g[0], lane / G * G);
-      if (!p.normalize) first = 0.f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        if (id[s] >= 0) g[s] -= first;
-        dot = fmaf(w[s], g[s], dot);
-        // 1 - sigmoid of the slot's logit, into its weight: w is done with.
-        if (p.sigmoid && id[s] >= 0)
-          w[s] *= rcp_ftz(1.f + ex2_ftz(elem_load(p.logits, p.type, t * p.ld + id[s]) * kLog2e));
-      }
-    }
-    const float mx = group_max<G>(lane_max(v));
-    const bool keep = mx > -INFINITY;
-    const float mxl = keep ? mx * kLog2e : 0.f;
-    Row<V> d;
-    float total = row_exp(v, keep ? mx : 0.f, mxl, d);
-    if (WEIGHTS) dot = group_sum<G>(dot);
-    if (!p.sigmoid) {
-      float2 fs = both(0.f);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) fs = __ffma2_rn(f(i), d.p[i], fs);
-      total = group_sum<G>(total);
-      const float fq = group_sum<G>(fs.x + fs.y);
-      const float inv = keep ? rcp_ftz(total) : 0.f;
-      // A row's share of every p: the z loss, the centring, the weights' dot.
-      const float every = dz * row_lse(mx, mxl, total) - fq * inv - (p.normalize ? 0.f : dot);
-      const float2 x = both(inv), y = both(every * inv);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) d.p[i] = __fmul2_rn(d.p[i], __ffma2_rn(f(i), x, y));
-    } else {
-      Row<V> ds;
-      float2 ns2 = both(0.f), fs = both(0.f);
-      row_sigmoid(v, d, mx, mxl, [&](int i, float2 s, float2 slope) {
-        ns2 = __fadd2_rn(ns2, s);
-        fs = __ffma2_rn(f(i), s, fs);
-        ds.p[i] = slope;
-      });
-      const float norm = group_sum<G>(ns2.x + ns2.y), fq = group_sum<G>(fs.x + fs.y);
-      const float qi = keep ? rcp_ftz(norm) : 0.f;
-      float zl = 0.f;
-      if (p.d_z) {
-        total = group_sum<G>(total);
-        zl = keep ? dz * row_lse(mx, mxl, total) * rcp_ftz(total) : 0.f;
-      }
-      const float2 x = both(qi), y = both(-fq * qi * qi), w2 = both(zl);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i)
-        d.p[i] = __ffma2_rn(ds.p[i], __ffma2_rn(f(i), x, y), __fmul2_rn(d.p[i], w2));
-    }
-    if (!keep) row_fill(d, 0.f);
-    if (!WEIGHTS && p.type != kElemF32 && p.vec_out == 8) {
-      // Nothing to add, and a lane's 16 or 32 bytes are whole sectors or
-      // halves that its next store fills: straight out (45 us against 54
-      // through shared memory at T = 131072, E = 256, sigmoid).
-#pragma unroll
-      for (int c = 0; c < V; c += 8) {
-        const float2* x = d.p + c / 2;
-        if (inside && e0 + c < E)
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.d_logits) + t * E + e0 + c) =
-              make_uint4(pack16(x[0].x, x[0].y, p.type), pack16(x[1].x, x[1].y, p.type),
-                         pack16(x[2].x, x[2].y, p.type), pack16(x[3].x, x[3].y, p.type));
-      }
-      continue;
-    }
-    __syncwarp();  // the last step's rows are stored
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q)
-      fours[four_at<V>(lane, q)] = make_float4(d.p[2 * q].x, d.p[2 * q].y, d.p[2 * q + 1].x, d.p[2 * q + 1].y);
-    __syncwarp();
-    if constexpr (WEIGHTS) {
-      const float off = p.normalize ? dot : 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        g[s] = w[s] * (g[s] - off);
-        // Slots of one expert (the caller's choice may repeat it) are added
-        // in slot order by the lowest of their lanes.
-        const int l = lane / G * G + id[s] / V;
-        const int key = id[s] >= 0 ? l * V + id[s] % V : -1 - lane;
-        const uint32_t peers = __match_any_sync(0xffffffffu, key);
-        bool mine = true;
-        if (__any_sync(0xffffffffu, peers != 1u << lane)) {
-          float sum = 0.f;
-          for (int x = 0; x < 32; ++x) {
-            const float other = __shfl_sync(0xffffffffu, g[s], x);
-            if (peers >> x & 1u) sum += other;
+        for (int s = 0; s < KS; ++s) {
+          if (id[s] < 0 || id[s] >= E) {  // dropped, whatever its gradient holds
+            id[s] = -1;
+            w[s] = g[s] = 0.f;
           }
-          g[s] = sum;
-          mine = lane == __ffs(peers) - 1;
         }
-        if (id[s] >= 0 && mine && keep)
-          reinterpret_cast<float*>(fours + four_at<V>(l, id[s] % V / 4))[id[s] % 4] += g[s];
-        __syncwarp();
+        float first = __shfl_sync(0xffffffffu, g[0], lane / G * G);
+        if (!p.normalize) first = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if (id[s] >= 0) g[s] -= first;
+          dot = fmaf(w[s], g[s], dot);
+          // 1 - sigmoid of the slot's logit, into its weight: w is done with.
+          if (p.sigmoid && id[s] >= 0)
+            w[s] *= rcp_ftz(1.f + ex2_ftz(elem_load(p.logits, p.type, t * p.ld + id[s]) * kLog2e));
+        }
       }
+      const float mx = group_max<G>(lane_max(v));
+      const bool keep = mx > -INFINITY;
+      const float mxl = keep ? mx * kLog2e : 0.f;
+      Row<V> d;
+      float total = row_exp(v, keep ? mx : 0.f, mxl, d);
+      if (WEIGHTS) dot = group_sum<G>(dot);
+      if (!p.sigmoid) {
+        float2 fs = both(0.f);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) fs = __ffma2_rn(f(i), d.p[i], fs);
+        total = group_sum<G>(total);
+        const float fq = group_sum<G>(fs.x + fs.y);
+        const float inv = keep ? rcp_ftz(total) : 0.f;
+        // A row's share of every p: the z loss, the centring, the weights' dot.
+        const float every = dz * row_lse(mx, mxl, total) - fq * inv - (p.normalize ? 0.f : dot);
+        const float2 x = both(inv), y = both(every * inv);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) d.p[i] = __fmul2_rn(d.p[i], __ffma2_rn(f(i), x, y));
+      } else {
+        Row<V> ds;
+        float2 ns2 = both(0.f), fs = both(0.f);
+        row_sigmoid(v, d, mx, mxl, [&](int i, float2 s, float2 slope) {
+          ns2 = __fadd2_rn(ns2, s);
+          fs = __ffma2_rn(f(i), s, fs);
+          ds.p[i] = slope;
+        });
+        const float norm = group_sum<G>(ns2.x + ns2.y), fq = group_sum<G>(fs.x + fs.y);
+        const float qi = keep ? rcp_ftz(norm) : 0.f;
+        float zl = 0.f;
+        if (p.d_z) {
+          total = group_sum<G>(total);
+          zl = keep ? dz * row_lse(mx, mxl, total) * rcp_ftz(total) : 0.f;
+        }
+        const float2 x = both(qi), y = both(-fq * qi * qi), w2 = both(zl);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+          d.p[i] = __ffma2_rn(ds.p[i], __ffma2_rn(f(i), x, y), __fmul2_rn(d.p[i], w2));
+      }
+      if (!keep) row_fill(d, 0.f);
+      if (!WEIGHTS && p.type != kElemF32 && p.vec_out == 8) {
+        // Nothing to add, and a lane's 16 or 32 bytes are whole sectors or
+        // halves that its next store fills: straight out (45 us against 54
+        // through shared memory at T = 131072, E = 256, sigmoid).
+#pragma unroll
+        for (int c = 0; c < V; c += 8) {
+          const float2* x = d.p + c / 2;
+          if (inside && e0 + c < E)
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.d_logits) + t * E + e0 + c) =
+                make_uint4(pack16(x[0].x, x[0].y, p.type), pack16(x[1].x, x[1].y, p.type),
+                           pack16(x[2].x, x[2].y, p.type), pack16(x[3].x, x[3].y, p.type));
+        }
+        continue;
+      }
+      __syncwarp();  // the last step's rows are stored
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q)
+        fours[four_at<V>(lane, q)] = make_float4(d.p[2 * q].x, d.p[2 * q].y, d.p[2 * q + 1].x, d.p[2 * q + 1].y);
+      __syncwarp();
+      if constexpr (WEIGHTS) {
+        const float off = p.normalize ? dot : 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          g[s] = w[s] * (g[s] - off);
+          // Slots of one expert (the caller's choice may repeat it) are added
+          // in slot order by the lowest of their lanes.
+          const int l = lane / G * G + id[s] / V;
+          const int key = id[s] >= 0 ? l * V + id[s] % V : -1 - lane;
+          const uint32_t peers = __match_any_sync(0xffffffffu, key);
+          bool mine = true;
+          if (__any_sync(0xffffffffu, peers != 1u << lane)) {
+            float sum = 0.f;
+            for (int x = 0; x < 32; ++x) {
+              const float other = __shfl_sync(0xffffffffu, g[s], x);
+              if (peers >> x & 1u) sum += other;
+            }
+            g[s] = sum;
+            mine = lane == __ffs(peers) - 1;
+          }
+          if (id[s] >= 0 && mine && keep)
+            reinterpret_cast<float*>(fours + four_at<V>(l, id[s] % V / 4))[id[s] % 4] += g[s];
+          __syncwarp();
+        }
+      }
+      rows_store<G, V>(fours, p.d_logits, p.type, p.vec_out, base, hi, E, lane);
     }
-    rows_store<G, V>(fours, p.d_logits, p.type, p.vec_out, base, hi, E, lane);
+    if (gridDim.x == (uint32_t)p.S * p.chunks) return;
+    __syncthreads();
+    if (threadIdx.x == 0) s_unit += gridDim.x;
+    __syncthreads();
+    unit = s_unit;
+    if (unit >= (uint32_t)p.S * p.chunks) return;
   }
 }
 
