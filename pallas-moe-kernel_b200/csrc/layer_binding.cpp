@@ -165,7 +165,8 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(shaped(*ids, r.T, k), "ids is ", ids->sizes(), ", expected [", r.T, ", ", k, "]");
     on(dev, *ids, "ids");
     TORCH_CHECK_TYPE(at::isIntegralType(ids->scalar_type(), false), "ids are ", ids->scalar_type(), ", not integers");
-    if (ids->scalar_type() == at::kLong) ids = ids->clamp(-1, r.E);  // far values stay out of range in 32 bits
+    // Far values stay out of range in 32 bits (as int64, those of uint64 are far or negative).
+    if (ids->element_size() == 8) ids = ids->to(at::kLong).clamp(-1, r.E);
     ids = ids->to(at::kInt).contiguous();
   }
   TORCH_CHECK_VALUE(1 <= k && k <= 16 && k <= r.E && r.E <= 1024, "k=", k, ", E=", r.E,
