@@ -429,7 +429,8 @@ enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
  * given_ids (T, k) or NULL: experts chosen by the caller, used in place of the
  * top k (an id outside [0, E) counts as -1; one id may come up twice).
  * E <= 1024, k <= min(16, E), T k < 2^31.  A NaN logit of a token that takes
- * part makes the losses NaN.  Workspace: moe_route_train_workspace_size
+ * part makes the losses NaN; one of +inf the z loss, and the balance loss of
+ * softmax scoring.  Workspace: moe_route_train_workspace_size
  * bytes, 256-byte aligned.  counters: moe_route_train_counters uint32 of
  * device memory that are zero at the first call which gets them; every call
  * leaves them zero.  Calls that may overlap need workspaces and counters of

@@ -28,9 +28,13 @@ static int route_lanes(int E) {
 }
 
 // Blocks per sequence: one for every step (a token per row group of the block)
-// while all of them are resident (3 blocks an SM at 80 registers a thread, 2 at
-// 128), else as few as share the steps evenly: a block with one token more than
-// its neighbours, or a second, short wave, costs a whole step.
+// while all of them are resident, else as few as share the steps evenly: a block
+// with one token more than its neighbours, or a second, short wave, costs a
+// whole step.  Resident is counted as 3 blocks an SM (80 registers a thread), 2
+// above 512 experts (128); the variants of up to 32 experts whose lanes hold
+// more than four slots have 2 as well and run what is over in a second wave.  A
+// sequence has a whole number of blocks: from 223 sequences on one each, which
+// leaves up to half of the slots empty.
 static int64_t route_chunks(int64_t seq_len, int64_t sequences, int E) {
   const int64_t step = kRouteWarps * (32 / route_lanes(E));
   const int64_t steps = std::max<int64_t>(1, (seq_len + step - 1) / step);

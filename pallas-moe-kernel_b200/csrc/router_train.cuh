@@ -562,8 +562,9 @@ constexpr int route_residents() {
 }
 
 // T = 131072, E = 256, k = 8, f32: 101 us; with given experts, bf16, sigmoid 62
-// (HBM's share 22 and 11).  Bounded by instruction issue, half of its slots at
-// 24 warps an SM, and by the special-function pipe.
+// (HBM's share 22 and 11).  Bounded by latency: 24 warps an SM with one row per
+// group of lanes in flight leave half of the issue slots empty while loads,
+// shuffles and special functions are waited for.
 template <int G, int V, int KMAX>
 __global__ void __launch_bounds__(kRouteThreads, route_residents<G, V, KMAX>()) route_train_kernel(const RouteParams p) {
   constexpr int TPW = 32 / G;                // tokens per warp and step
